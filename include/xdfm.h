@@ -17,7 +17,7 @@
  *    device (workspaces are sized by *_workspace_bytes and passed in).
  *  - `stream` is a hipStream_t passed as void*; all device entry points only
  *    enqueue work on it and return without synchronising.
- *  - all floating point tensors are IEEE fp32, row-major, densely packed.
+ *  - all floating point tensors are IEEE fp32, row-major, densely packed, where nothing else is said.
  *  - `err_flag` is a device int32 the kernels OR error bits into
  *    (XDFM_DEVERR_*); the host reads it at its next natural sync point.
  */
@@ -65,6 +65,11 @@ extern "C" {
 #define XDFM_ACT_SIGMOID 2
 #define XDFM_ACT_TANH 3
 #define XDFM_ACT_ELU 4
+
+/* element type of the entry points that serve several */
+#define XDFM_F32 0
+#define XDFM_BF16 1
+#define XDFM_F16 2
 
 int xdfm_abi_version(void);
 const char* xdfm_last_error(void);
@@ -367,6 +372,68 @@ int xdfm_dense_update(float* param, const float* grad, float* slot_m, float* slo
 int xdfm_dense_reg_loss(const float* param, int32_t n_seg, const int64_t* seg_off, const float* seg_l2,
                         const float* seg_l1, const float* seg_norm_l2, float* stats, float* reg_loss,
                         int32_t accumulate_reg_loss, void* stream);
+
+/* ------------------------------------------------------------------------
+ * AdamW over many tensors at once, states in 32 or in 8 bits.  No counterpart in the reference (its
+ * optimizers, base_model.py:283-302, have no decoupled weight decay and fp32 slots).
+ *   m <- beta1 m + (1 - beta1) g      v <- beta2 v + (1 - beta2) g^2
+ *   p <- p - lr weight_decay p - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * The tensors are described once (xdfm_adamw_plan): the plan is an image in host memory that the caller
+ * copies to the device and keeps for as long as the tensors stay where they are.  A step is then one
+ * launch, however many tensors there are.
+ *
+ * 32-bit states: slot_m, slot_v fp32 [n].
+ * 8-bit states: slot_m, slot_v uint8 [n], scale_m, scale_v uint8 [ceil(n / 64)], all of them zero before
+ * the first step.  A block is 64 consecutive elements of a tensor; its scale byte s is the biased
+ * exponent of its largest magnitude (48 at least).  A code's size (m: 7 bits under a sign bit, v: 8) is
+ * e * 8 + f and stands for f units (e = 0) or (8 + f) 2^(e-1) units, a unit being 2^(s - 143) for m and
+ * 2^(s - 159) for v: 4 significant bits over 17 binades of m, 33 of v.  Values are rounded up with the
+ * probability that the cut-off part is of the last kept bit, out of 16 random bits of (seed, step, tensor's
+ * position in the plan, element): to the nearest, a v that moves by a thousandth of itself per step would
+ * never move.  A v > 0 never becomes 0.  The step itself uses m and v before they are rounded.  A block with
+ * a value that is not finite gets the scale 255 and reads as NaN from then on.
+ * ---------------------------------------------------------------------- */
+typedef struct xdfm_adamw_tensor {
+  float* param;        /* fp32 [n], device */
+  const void* grad;    /* [n] of grad_dtype */
+  void* slot_m;        /* fp32 [n] or codes uint8 [n] */
+  void* slot_v;
+  uint8_t* scale_m;    /* uint8 [ceil(n / 64)]; NULL with 32-bit states */
+  uint8_t* scale_v;
+  int64_t n;           /* elements; 0: skipped */
+  float weight_decay;
+  int32_t grad_dtype;  /* XDFM_F32, XDFM_BF16 or XDFM_F16 */
+} xdfm_adamw_tensor;
+
+typedef struct xdfm_adamw_plan_info {
+  int64_t bytes;       /* of the plan's image */
+  int64_t chunks;
+  int64_t elements;    /* of all tensors */
+  int32_t state_bits;  /* 32 or 8 */
+  int32_t chunk_elems;
+} xdfm_adamw_plan_info;
+
+typedef struct xdfm_adamw_args {
+  double lr, beta1, beta2, eps;
+  const float* opt_state; /* NULL, or device: t = opt_state[3] (xdfm_opt_advance), so that a step can be captured */
+  int64_t step;           /* t, 1 for the first step; used where opt_state is NULL */
+  uint64_t seed;          /* of the rounding of 8-bit states */
+} xdfm_adamw_args;
+
+/* Host only.  image = NULL: fills *info alone.  Otherwise `image` (host, 8-byte aligned, image_bytes >= the
+ * info->bytes of a call without it) receives the plan and *info is filled again.  Refused: null pointers of tensors
+ * with elements, misaligned fp32 / 16-bit pointers, and tensors of which one is written where another one is
+ * written or read. */
+int xdfm_adamw_plan(const xdfm_adamw_tensor* tensors, int32_t n_tensors, int32_t state_bits, void* image,
+                    size_t image_bytes, xdfm_adamw_plan_info* info);
+/* One step of all tensors.  plan: the image in device memory (8-byte aligned), info: as xdfm_adamw_plan gave it. */
+int xdfm_adamw_step(const void* plan, const xdfm_adamw_plan_info* info, const xdfm_adamw_args* args, void* stream);
+/* 8-bit states as the values they stand for: m, v bf16 [info->elements] (4 significant bits times a power of two:
+ * bf16 holds them exactly), the plan's tensors one behind the other. */
+int xdfm_adamw_state_read(const void* plan, const xdfm_adamw_plan_info* info, uint16_t* m, uint16_t* v, void* stream);
+/* 8-bit states from values, rounded to the nearest (v > 0 not to 0): m, v fp32 [info->elements]. */
+int xdfm_adamw_state_write(const void* plan, const xdfm_adamw_plan_info* info, const float* m, const float* v,
+                           void* stream);
 
 /* ------------------------------------------------------------------------
  * Compressed Interaction Network, one layer.   xDeepFM.py:191-267
@@ -710,6 +777,31 @@ int xdfm_bn_bwd_sums(const float* x, const float* y, const float* dy, int64_t B,
 int xdfm_bn_bwd_apply(const float* x, const float* y, const float* dy, int64_t B, int32_t C, int32_t I,
                       int64_t n_total, const float* gamma, const float* stats, int32_t act,
                       const float* sum_gamma, const float* sum_beta, float* dx, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Layer norm of the rows of a matrix with the activation behind it, for the optional enable_LN branch of
+ * the DNN tower (no counterpart in the reference, which normalises over the batch, xDeepFM.py:497-503).
+ *   xhat = (x - mean) * rstd, mean and rstd = 1 / sqrt(var + eps) over the row's `cols` elements (biased
+ *   variance);  y = act(gamma * xhat + beta)
+ *   x, y, dy, dx: [rows, cols] of `dtype` (XDFM_F32, XDFM_BF16, XDFM_F16), *_stride elements (cols at least)
+ *     between consecutive rows, any alignment of the type; what lies between rows is neither read nor
+ *     written.  gamma, beta, dgamma, dbeta [cols] and stats are fp32, as is all arithmetic.
+ *   stats [2, rows] (NULL ok): mean, then rstd, for the backward pass.
+ * y may be x (same address and stride); dx may be dy or x.
+ * Backward, from x and stats (y is not read):  du = dy * act'(u), u = gamma * xhat + beta (relu: on where u is
+ * positive exactly);  t = du * gamma;  dx = rstd * (t - mean_row(t) - xhat * mean_row(t * xhat));
+ *   dgamma[c] = sum_rows du * xhat, dbeta[c] = sum_rows du (written; the order of the sums is fixed by the
+ *   sizes: two runs agree in every bit).
+ *   workspace: device float scratch of xdfm_layer_norm_bwd_workspace_floats(...) elements (16-byte aligned),
+ *     of its own for every call that may be under way at the same time.
+ * ---------------------------------------------------------------------- */
+int xdfm_layer_norm_fwd(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int32_t cols, const float* gamma,
+                        const float* beta, float eps, int32_t act, void* y, int64_t y_stride, float* stats,
+                        void* stream);
+int xdfm_layer_norm_bwd_workspace_floats(int64_t rows, int32_t cols, size_t* floats);
+int xdfm_layer_norm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, int32_t dtype, int64_t rows,
+                        int32_t cols, const float* gamma, const float* beta, const float* stats, int32_t act, void* dx,
+                        int64_t dx_stride, float* dgamma, float* dbeta, float* workspace, void* stream);
 
 /* softmax activation (`_activate`, base_model.py:343-344: tf.nn.softmax over the last axis), the
  * one activation the fused forms above do not carry: run the layer with the identity and then

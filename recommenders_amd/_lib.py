@@ -117,6 +117,48 @@ class CinPackJob(ctypes.Structure):
     ]
 
 
+class AdamWTensor(ctypes.Structure):
+    """struct xdfm_adamw_tensor"""
+
+    _fields_ = [
+        ("param", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("slot_m", ctypes.c_void_p),
+        ("slot_v", ctypes.c_void_p),
+        ("scale_m", ctypes.c_void_p),
+        ("scale_v", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+        ("weight_decay", ctypes.c_float),
+        ("grad_dtype", ctypes.c_int32),
+    ]
+
+
+class AdamWPlanInfo(ctypes.Structure):
+    """struct xdfm_adamw_plan_info"""
+
+    _fields_ = [
+        ("bytes", ctypes.c_int64),
+        ("chunks", ctypes.c_int64),
+        ("elements", ctypes.c_int64),
+        ("state_bits", ctypes.c_int32),
+        ("chunk_elems", ctypes.c_int32),
+    ]
+
+
+class AdamWArgs(ctypes.Structure):
+    """struct xdfm_adamw_args"""
+
+    _fields_ = [
+        ("lr", ctypes.c_double),
+        ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("opt_state", ctypes.c_void_p),
+        ("step", ctypes.c_int64),
+        ("seed", ctypes.c_uint64),
+    ]
+
+
 class BatchInfo(ctypes.Structure):
     """struct xdfm_ffm_batch_info"""
 
@@ -170,6 +212,10 @@ SIGNATURES = {
     "xdfm_dense_update": [_P, _P, _P, _P, _I32, _P, _P, _P, _P, ctypes.POINTER(OptArgs), _P, _P,
                           _I32, _P],
     "xdfm_dense_reg_loss": [_P, _I32, _P, _P, _P, _P, _P, _P, _I32, _P],
+    "xdfm_adamw_plan": [ctypes.POINTER(AdamWTensor), _I32, _I32, _P, _SZ, ctypes.POINTER(AdamWPlanInfo)],
+    "xdfm_adamw_step": [_P, ctypes.POINTER(AdamWPlanInfo), ctypes.POINTER(AdamWArgs), _P],
+    "xdfm_adamw_state_read": [_P, ctypes.POINTER(AdamWPlanInfo), _P, _P, _P],
+    "xdfm_adamw_state_write": [_P, ctypes.POINTER(AdamWPlanInfo), _P, _P, _P],
     "xdfm_cin_fwd_workspace_floats": [_I64, _I32, _I32, _I32, _I32, _PSZ],
     "xdfm_cin_fwd": [_P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _P, _P, _I32, _I32, _P, _P],
     "xdfm_cin_bwd_workspace_floats": [_I64, _I32, _I32, _I32, _I32, _PSZ],
@@ -200,6 +246,9 @@ SIGNATURES = {
     "xdfm_cin_pool_pack": [_P, _I32, _I32, _I32, _I32, _I32, _P, _P],
     "xdfm_cin_pool_unpack": [_P, _I32, _I32, _I32, _I32, _I32, _P, _P],
     "xdfm_bn_fwd": [_P, _I64, _I32, _I32, _P, _P, _P, _P, ctypes.c_float, ctypes.c_float, _I32, _I32, _P, _P, _P],
+    "xdfm_layer_norm_fwd": [_P, _I64, _I32, _I64, _I32, _P, _P, ctypes.c_float, _I32, _P, _I64, _P, _P],
+    "xdfm_layer_norm_bwd_workspace_floats": [_I64, _I32, _PSZ],
+    "xdfm_layer_norm_bwd": [_P, _I64, _P, _I64, _I32, _I64, _I32, _P, _P, _P, _I32, _P, _I64, _P, _P, _P, _P],
     "xdfm_softmax_fwd": [_P, _I64, _I32, _I32, _P, _P],
     "xdfm_softmax_bwd": [_P, _P, _I64, _I32, _I32, _P, _P],
     "xdfm_bn_bwd": [_P, _P, _P, _I64, _I32, _I32, _P, _P, _I32, _P, _P, _P, _P],

@@ -1,0 +1,374 @@
+// AdamW over many tensors at once, states in 32 or in 8 bits (xdfm_adamw_*, include/xdfm.h).
+//
+//   m <- b1 m + (1 - b1) g,  v <- b2 v + (1 - b2) g^2
+//   p <- p - lr wd p - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// The plan is an array of chunks: runs of at most chunk_elems elements of one tensor with their addresses, so that
+// a block needs one record and no search, and tensors of one element and of 10^8 share a launch.
+// The codes of the 8-bit states: a value scaled by a power of two so that the largest of its block has the
+// exponent field 14 (m) or 30 (v) as a float; the float's bits from the third mantissa bit up are then the code, and
+// what lies below is cut off after random bits were added to it.  Values under 2^-126 of that scale are denormal
+// floats, whose bits go on being the value in units: the same shift codes them too.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "xdfm_common.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlock = 64;  // elements that share a scale
+constexpr int kChunk = 4096;
+constexpr int kScaleMin = 48;  // units stay normal floats: 2^(48 - 159)
+constexpr uint32_t kMul1 = 0x9E3779B1u;  // 2^32 / golden ratio
+constexpr uint32_t kMul2 = 0x6A09E667u;  // the fraction of sqrt(2)
+
+struct Chunk {
+  float* p;
+  const void* g;
+  void* m;
+  void* v;
+  uint8_t* sm;
+  uint8_t* sv;
+  int64_t start;  // of the chunk in its tensor (a multiple of kBlock)
+  int64_t out;    // of the chunk in the tensors laid one behind the other
+  int32_t count;
+  int32_t tensor;
+  float wd;
+  int32_t gtype;
+};
+static_assert(sizeof(Chunk) == 80, "the plan's record");
+
+struct Args {
+  float lr, b1, omb1, b2, omb2, eps;
+  float log_b1, log_b2;     // for t from the device
+  float step, inv_root;     // lr / (1 - b1^t), 1 / sqrt(1 - b2^t) for t from the host
+  const float* state;
+  uint32_t seed_lo, seed_hi, t;
+};
+
+struct Step {
+  float size, inv_root;
+  uint32_t t;
+};
+
+__device__ __forceinline__ Step step_of(const Args& a) {
+  if (!a.state) return {a.step, a.inv_root, a.t};
+  const float t = a.state[3];
+  return {a.lr / -expm1f(t * a.log_b1), 1.f / sqrtf(-expm1f(t * a.log_b2)), (uint32_t)t};
+}
+
+__device__ __forceinline__ float grad_of(const void* g, int type, int64_t i) {
+  if (type == XDFM_F32) return ((const float*)g)[i];
+  if (type == XDFM_BF16) return (float)((const __bf16*)g)[i];
+  return (float)((const _Float16*)g)[i];
+}
+
+// (multiplications and additions are not contracted in this build: m and v are the two products' sum)
+__device__ __forceinline__ float update(float p, float g, float& m, float& v, const Args& a, const Step& s, float wd) {
+  m = m * a.b1 + g * a.omb1;
+  v = v * a.b2 + (g * g) * a.omb2;
+  return (p - (a.lr * wd) * p) - s.size * m / (sqrtf(v) * s.inv_root + a.eps);
+}
+
+__device__ __forceinline__ uint32_t mix(uint32_t a, uint32_t b) { return (a ^ (a >> 15)) * kMul1 + b; }
+
+// keys of a tensor's random bits at a step
+__device__ __forceinline__ uint2 keys_of(const Args& a, uint32_t t, int tensor, int64_t i) {
+  const uint32_t k = mix(mix(mix(a.seed_lo, a.seed_hi), t), (uint32_t)tensor);
+  return make_uint2(mix(k, 1u), mix(k, 2u + (uint32_t)(i >> 32)));
+}
+
+__device__ __forceinline__ uint32_t random_bits(uint2 k, uint32_t i) {
+  uint32_t a = (i + k.x) * kMul1;
+  a = (a ^ (a >> 15) ^ k.y) * kMul2;
+  return a ^ (a >> 16);
+}
+
+// largest magnitude of a block (as bits: NaN above infinity above the rest) -> its scale byte
+__device__ __forceinline__ int scale_of(uint32_t top) {
+  const int e = (int)(top >> 23);
+  return e < kScaleMin ? kScaleMin : e;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) x = max(x, (uint32_t)__shfl_xor((int)x, m));
+  return x;
+}
+
+__device__ __forceinline__ uint32_t code_of(float size, int shift, uint32_t r20) {
+  return (__float_as_uint(ldexpf(size, shift)) + r20) >> 20;
+}
+__device__ __forceinline__ uint8_t code_m(float x, int s, uint32_t r20) {
+  return (uint8_t)(code_of(fabsf(x), 14 - s, r20) | (__float_as_uint(x) >> 24 & 0x80u));
+}
+__device__ __forceinline__ uint8_t code_v(float x, int s, uint32_t r20) {
+  const uint32_t c = code_of(x, 30 - s, r20);
+  return (uint8_t)(c ? c : x > 0.f);
+}
+__device__ __forceinline__ float value_m(uint32_t c, int s) {
+  const float x = __uint_as_float((c & 0x7Fu) << 20 | (c & 0x80u) << 24);
+  return s == 255 ? __uint_as_float(0x7FC00000u) : ldexpf(x, s - 14);
+}
+__device__ __forceinline__ float value_v(uint32_t c, int s) {
+  return s == 255 ? __uint_as_float(0x7FC00000u) : ldexpf(__uint_as_float(c << 20), s - 30);
+}
+
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const Chunk* __restrict__ chunks, Args a) {
+  const Chunk c = chunks[blockIdx.x];
+  const Step s = step_of(a);
+  float *m = (float*)c.m, *v = (float*)c.v;
+  for (int i = threadIdx.x; i < c.count; i += kThreads) {
+    float mi = m[i], vi = v[i];
+    c.p[i] = update(c.p[i], grad_of(c.g, c.gtype, i), mi, vi, a, s, c.wd);
+    m[i] = mi;
+    v[i] = vi;
+  }
+}
+
+// a wave per block of 64
+__global__ __launch_bounds__(kThreads) void adamw8_kernel(const Chunk* __restrict__ chunks, Args a) {
+  const Chunk c = chunks[blockIdx.x];
+  const Step s = step_of(a);
+  const uint2 key = keys_of(a, s.t, c.tensor, c.start);
+  uint8_t *m = (uint8_t*)c.m, *v = (uint8_t*)c.v;
+  for (int i0 = threadIdx.x & ~63; i0 < c.count; i0 += kThreads) {
+    const int b = i0 / kBlock, i = i0 + (threadIdx.x & 63);
+    const bool in = i < c.count;
+    float mi = 0.f, vi = 0.f;
+    if (in) {
+      mi = value_m(m[i], c.sm[b]);
+      vi = value_v(v[i], c.sv[b]);
+      c.p[i] = update(c.p[i], grad_of(c.g, c.gtype, i), mi, vi, a, s, c.wd);
+    }
+    const int sm = scale_of(wave_max(__float_as_uint(fabsf(mi)))), sv = scale_of(wave_max(__float_as_uint(fabsf(vi))));
+    if (in) {
+      const uint32_t r = random_bits(key, (uint32_t)(c.start + i));
+      m[i] = code_m(mi, sm, ((r & 0xFFFFu) << 4) + 8u);
+      v[i] = code_v(vi, sv, ((r >> 16) << 4) + 8u);
+      if (i == i0) {
+        c.sm[b] = (uint8_t)sm;
+        c.sv[b] = (uint8_t)sv;
+      }
+    }
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void adamw_state_read_kernel(const Chunk* __restrict__ chunks,
+                                                                    __bf16* __restrict__ out_m,
+                                                                    __bf16* __restrict__ out_v) {
+  const Chunk c = chunks[blockIdx.x];
+  const uint8_t *m = (const uint8_t*)c.m, *v = (const uint8_t*)c.v;
+  for (int i = threadIdx.x; i < c.count; i += kThreads) {
+    out_m[c.out + i] = (__bf16)value_m(m[i], c.sm[i / kBlock]);
+    out_v[c.out + i] = (__bf16)value_v(v[i], c.sv[i / kBlock]);
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void adamw_state_write_kernel(const Chunk* __restrict__ chunks,
+                                                                     const float* __restrict__ in_m,
+                                                                     const float* __restrict__ in_v) {
+  const Chunk c = chunks[blockIdx.x];
+  uint8_t *m = (uint8_t*)c.m, *v = (uint8_t*)c.v;
+  for (int i0 = threadIdx.x & ~63; i0 < c.count; i0 += kThreads) {
+    const int b = i0 / kBlock, i = i0 + (threadIdx.x & 63);
+    const bool in = i < c.count;
+    const float mi = in ? in_m[c.out + i] : 0.f, vi = in ? in_v[c.out + i] : 0.f;
+    const int sm = scale_of(wave_max(__float_as_uint(fabsf(mi)))), sv = scale_of(wave_max(__float_as_uint(fabsf(vi))));
+    if (in) {
+      m[i] = code_m(mi, sm, 1u << 19);
+      v[i] = code_v(vi, sv, 1u << 19);
+      if (i == i0) {
+        c.sm[b] = (uint8_t)sm;
+        c.sv[b] = (uint8_t)sv;
+      }
+    }
+  }
+}
+
+struct Range {
+  uintptr_t beg, end;
+  int tensor;
+};
+
+// every range that is written lies apart from every other one, and from those that are read
+int check_apart(const xdfm_adamw_tensor* t, int n, int bits) {
+  std::vector<Range> written, read;
+  const size_t size = bits == 32 ? 4 : 1;
+  auto put = [](std::vector<Range>& to, const void* p, size_t bytes, int k) {
+    to.push_back({(uintptr_t)p, (uintptr_t)p + bytes, k});
+  };
+  for (int k = 0; k < n; ++k) {
+    if (t[k].n == 0) continue;
+    const size_t e = (size_t)t[k].n, blocks = (e + kBlock - 1) / kBlock;
+    put(written, t[k].param, 4 * e, k);
+    put(written, t[k].slot_m, size * e, k);
+    put(written, t[k].slot_v, size * e, k);
+    if (bits == 8) {
+      put(written, t[k].scale_m, blocks, k);
+      put(written, t[k].scale_v, blocks, k);
+    }
+    put(read, t[k].grad, (t[k].grad_dtype == XDFM_F32 ? 4 : 2) * e, k);
+  }
+  auto before = [](const Range& x, const Range& y) { return x.beg < y.beg; };
+  std::sort(written.begin(), written.end(), before);
+  for (size_t i = 1; i < written.size(); ++i)
+    XDFM_REQUIRE(written[i - 1].end <= written[i].beg, "xdfm_adamw_plan: tensors %d and %d overlap where they are written",
+                 written[i - 1].tensor, written[i].tensor);
+  for (const Range& r : read) {
+    auto after = std::lower_bound(written.begin(), written.end(), r, before);
+    XDFM_REQUIRE(after == written.end() || r.end <= after->beg, "xdfm_adamw_plan: the gradient of tensor %d lies in what "
+                 "the step writes of tensor %d", r.tensor, after->tensor);
+    XDFM_REQUIRE(after == written.begin() || (after - 1)->end <= r.beg, "xdfm_adamw_plan: the gradient of tensor %d lies "
+                 "in what the step writes of tensor %d", r.tensor, (after - 1)->tensor);
+  }
+  return XDFM_OK;
+}
+
+int make_plan(const xdfm_adamw_tensor* t, int n, int bits, Chunk* image, xdfm_adamw_plan_info* info) {
+  int64_t chunks = 0, out = 0;
+  for (int k = 0; k < n; ++k) {
+    const xdfm_adamw_tensor& x = t[k];
+    XDFM_REQUIRE(x.n >= 0 && x.n <= (int64_t)1 << 44, "xdfm_adamw_plan: tensor %d has %lld elements", k, (long long)x.n);
+    XDFM_REQUIRE(x.grad_dtype == XDFM_F32 || x.grad_dtype == XDFM_BF16 || x.grad_dtype == XDFM_F16,
+                 "xdfm_adamw_plan: tensor %d: unknown gradient type %d", k, x.grad_dtype);
+    XDFM_REQUIRE(x.weight_decay >= 0.f && std::isfinite(x.weight_decay),
+                 "xdfm_adamw_plan: tensor %d: weight_decay has to be finite and not negative", k);
+    if (x.n == 0) continue;
+    XDFM_REQUIRE(x.param && x.grad && x.slot_m && x.slot_v, "xdfm_adamw_plan: tensor %d: null argument", k);
+    XDFM_REQUIRE(bits == 32 || (x.scale_m && x.scale_v), "xdfm_adamw_plan: tensor %d: 8-bit states need their scales", k);
+    XDFM_REQUIRE(bits == 8 || (!x.scale_m && !x.scale_v), "xdfm_adamw_plan: tensor %d: 32-bit states have no scales", k);
+    XDFM_REQUIRE(((uintptr_t)x.param & 3) == 0 && ((uintptr_t)x.grad & (x.grad_dtype == XDFM_F32 ? 3 : 1)) == 0 &&
+                     (bits == 8 || (((uintptr_t)x.slot_m | (uintptr_t)x.slot_v) & 3) == 0),
+                 "xdfm_adamw_plan: tensor %d: misaligned pointer", k);
+    const int gsize = x.grad_dtype == XDFM_F32 ? 4 : 2, ssize = bits == 32 ? 4 : 1;
+    for (int64_t at = 0; at < x.n; at += kChunk, ++chunks) {
+      if (!image) {
+        const int64_t more = (x.n - 1) / kChunk;  // counted, not walked
+        chunks += more;
+        at += more * kChunk;
+        continue;
+      }
+      Chunk& c = image[chunks];
+      c.p = x.param + at;
+      c.g = (const char*)x.grad + at * gsize;
+      c.m = (char*)x.slot_m + at * ssize;
+      c.v = (char*)x.slot_v + at * ssize;
+      c.sm = x.scale_m ? x.scale_m + at / kBlock : nullptr;
+      c.sv = x.scale_v ? x.scale_v + at / kBlock : nullptr;
+      c.start = at;
+      c.out = out + at;
+      c.count = (int32_t)std::min<int64_t>(kChunk, x.n - at);
+      c.tensor = k;
+      c.wd = x.weight_decay;
+      c.gtype = x.grad_dtype;
+    }
+    out += x.n;
+  }
+  XDFM_REQUIRE(chunks < (int64_t)1 << 31, "xdfm_adamw_plan: too many elements");
+  info->bytes = chunks * (int64_t)sizeof(Chunk);
+  info->chunks = chunks;
+  info->elements = out;
+  info->state_bits = bits;
+  info->chunk_elems = kChunk;
+  return XDFM_OK;
+}
+
+int check_plan(const char* who, const void* plan, const xdfm_adamw_plan_info* info) {
+  XDFM_REQUIRE(info, "%s: null argument", who);
+  XDFM_REQUIRE((info->state_bits == 32 || info->state_bits == 8) && info->chunk_elems == kChunk && info->chunks >= 0 &&
+                   info->chunks < (int64_t)1 << 31 && info->bytes == info->chunks * (int64_t)sizeof(Chunk),
+               "%s: *info is not what xdfm_adamw_plan gave", who);
+  XDFM_REQUIRE(info->chunks == 0 || plan, "%s: null argument", who);
+  XDFM_REQUIRE(((uintptr_t)plan & 7) == 0, "%s: misaligned plan", who);
+  return XDFM_OK;
+}
+
+}  // namespace
+
+extern "C" int xdfm_adamw_plan(const xdfm_adamw_tensor* tensors, int32_t n_tensors, int32_t state_bits, void* image,
+                               size_t image_bytes, xdfm_adamw_plan_info* info) {
+  XDFM_REQUIRE(info && n_tensors >= 0 && (tensors || n_tensors == 0), "xdfm_adamw_plan: bad argument");
+  XDFM_REQUIRE(state_bits == 32 || state_bits == 8, "xdfm_adamw_plan: states have 32 or 8 bits, not %d", state_bits);
+  XDFM_REQUIRE(((uintptr_t)image & 7) == 0, "xdfm_adamw_plan: misaligned image");
+  try {
+    const int rc = make_plan(tensors, n_tensors, state_bits, nullptr, info);
+    if (rc) return rc;
+    if (!image) return check_apart(tensors, n_tensors, state_bits);
+    if (image_bytes < (size_t)info->bytes)
+      return xdfm::fail(XDFM_E_WORKSPACE, "xdfm_adamw_plan: the image takes %lld bytes", (long long)info->bytes);
+    return make_plan(tensors, n_tensors, state_bits, (Chunk*)image, info);
+  } catch (const std::exception& e) {
+    return xdfm::fail(XDFM_E_INVALID, "xdfm_adamw_plan: %s", e.what());
+  }
+}
+
+extern "C" int xdfm_adamw_step(const void* plan, const xdfm_adamw_plan_info* info, const xdfm_adamw_args* args,
+                               void* stream) {
+  const int rc = check_plan("xdfm_adamw_step", plan, info);
+  if (rc) return rc;
+  XDFM_REQUIRE(args, "xdfm_adamw_step: null argument");
+  XDFM_REQUIRE(std::isfinite(args->lr) && args->lr >= 0, "xdfm_adamw_step: lr has to be finite and not negative");
+  XDFM_REQUIRE(args->beta1 >= 0 && args->beta1 < 1 && args->beta2 >= 0 && args->beta2 < 1,
+               "xdfm_adamw_step: beta1 and beta2 have to lie in [0, 1)");
+  XDFM_REQUIRE(std::isfinite(args->eps) && (float)args->eps > 0.f, "xdfm_adamw_step: eps has to be positive");
+  XDFM_REQUIRE(args->opt_state || args->step >= 1, "xdfm_adamw_step: steps count from 1");
+  if (info->chunks == 0) return XDFM_OK;
+  Args a;
+  a.lr = (float)args->lr;
+  a.b1 = (float)args->beta1;
+  a.omb1 = (float)(1.0 - args->beta1);
+  a.b2 = (float)args->beta2;
+  a.omb2 = (float)(1.0 - args->beta2);
+  a.eps = (float)args->eps;
+  a.log_b1 = (float)std::log(args->beta1);
+  a.log_b2 = (float)std::log(args->beta2);
+  a.state = args->opt_state;
+  a.step = a.inv_root = 0.f;
+  a.t = 0;
+  if (!a.state) {
+    const double t = (double)args->step;
+    a.step = (float)(args->lr / (1.0 - std::pow(args->beta1, t)));
+    a.inv_root = (float)(1.0 / std::sqrt(1.0 - std::pow(args->beta2, t)));
+    a.t = (uint32_t)args->step;
+  }
+  a.seed_lo = (uint32_t)args->seed;
+  a.seed_hi = (uint32_t)(args->seed >> 32);
+  if (info->state_bits == 32)
+    XDFM_LAUNCH("adamw_kernel", stream, adamw_kernel, dim3((unsigned)info->chunks), dim3(kThreads), 0,
+                (const Chunk*)plan, a);
+  else
+    XDFM_LAUNCH("adamw8_kernel", stream, adamw8_kernel, dim3((unsigned)info->chunks), dim3(kThreads), 0,
+                (const Chunk*)plan, a);
+  XDFM_LAUNCH_CHECK();
+  return XDFM_OK;
+}
+
+extern "C" int xdfm_adamw_state_read(const void* plan, const xdfm_adamw_plan_info* info, uint16_t* m, uint16_t* v,
+                                     void* stream) {
+  const int rc = check_plan("xdfm_adamw_state_read", plan, info);
+  if (rc) return rc;
+  XDFM_REQUIRE(info->state_bits == 8, "xdfm_adamw_state_read: 32-bit states are values as they stand");
+  if (info->chunks == 0) return XDFM_OK;
+  XDFM_REQUIRE(m && v && (((uintptr_t)m | (uintptr_t)v) & 1) == 0, "xdfm_adamw_state_read: null or misaligned output");
+  XDFM_LAUNCH("adamw_state_read_kernel", stream, adamw_state_read_kernel, dim3((unsigned)info->chunks), dim3(kThreads),
+              0, (const Chunk*)plan, (__bf16*)m, (__bf16*)v);
+  XDFM_LAUNCH_CHECK();
+  return XDFM_OK;
+}
+
+extern "C" int xdfm_adamw_state_write(const void* plan, const xdfm_adamw_plan_info* info, const float* m,
+                                      const float* v, void* stream) {
+  const int rc = check_plan("xdfm_adamw_state_write", plan, info);
+  if (rc) return rc;
+  XDFM_REQUIRE(info->state_bits == 8, "xdfm_adamw_state_write: 32-bit states are values as they stand");
+  if (info->chunks == 0) return XDFM_OK;
+  XDFM_REQUIRE(m && v && (((uintptr_t)m | (uintptr_t)v) & 3) == 0, "xdfm_adamw_state_write: null or misaligned input");
+  XDFM_LAUNCH("adamw_state_write_kernel", stream, adamw_state_write_kernel, dim3((unsigned)info->chunks),
+              dim3(kThreads), 0, (const Chunk*)plan, m, v);
+  XDFM_LAUNCH_CHECK();
+  return XDFM_OK;
+}
