@@ -20,6 +20,11 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
 
+// How rows are read and written.  kStream: past the caches.  A pass over more than the Infinity Cache holds (256 MB)
+// leaves nothing in it that the next kernel would find (1024 x 65536 fp32 forward 98 -> 91 us, 512 x 65536 backward 80
+// -> 72), a smaller one might (and gains nothing: 1001 x 4099 fp16 9.0 -> 9.35).
+enum { kPlain, kStream };
+
 // The pieces of a row that a thread holds.  Element j of piece k is column c[k] + j and counts where j >= skip[k]:
 // a piece that would pass the row's end is moved back to end there and leaves out what its neighbour holds, so that
 // loads need no condition (one inside the loop would wait for the loads under way); one that lies behind the end
@@ -52,11 +57,14 @@ __device__ __forceinline__ void mask(float (&v)[V], int skip) {
   for (int j = 0; j < V; ++j) v[j] = j >= skip ? v[j] : 0.f;
 }
 
-template <typename T, int NV>
+template <int MODE, typename T, int NV>
 __device__ __forceinline__ void load_row(const T* row, const Pieces<T, NV>& at, bool tiny, u32x4 (&w)[NV]) {
   if (!tiny) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) w[k] = *reinterpret_cast<const u32x4_any*>(row + at.c[k]);
+    for (int k = 0; k < NV; ++k) {
+      const u32x4_any* from = reinterpret_cast<const u32x4_any*>(row + at.c[k]);
+      w[k] = MODE == kStream ? __builtin_nontemporal_load(from) : *from;
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -85,7 +93,7 @@ __device__ __forceinline__ void load_weights(const float* __restrict__ w, const 
 }
 
 // what counts of V elements to `to` (column c)
-template <typename T, int V>
+template <int MODE, typename T, int V>
 __device__ __forceinline__ void store_piece(T* to, int skip, const float (&v)[V]) {
   T e[V];
 #pragma unroll
@@ -95,7 +103,10 @@ __device__ __forceinline__ void store_piece(T* to, int skip, const float (&v)[V]
     for (int i = 0; i < V * (int)sizeof(T) / 16; ++i) {
       u32x4 w;
       __builtin_memcpy(&w, (const char*)e + 16 * i, 16);
-      reinterpret_cast<u32x4_any*>(to)[i] = w;
+      if (MODE == kStream)
+        __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(to) + i);
+      else
+        reinterpret_cast<u32x4_any*>(to)[i] = w;
     }
   } else {
 #pragma unroll
@@ -127,6 +138,18 @@ __device__ __forceinline__ float group_sum(float v) {
     v = __uint_as_float(h[0]) + __uint_as_float(h[1]);
   }
   return v;
+}
+
+// sum over the lanes of a wave that are equal modulo G, the same in each of them
+template <int G>
+__device__ __forceinline__ float groups_sum(float v) {
+  if (G <= 8) v += dpp<0x128>(v);  // turned by 8 within 16
+  if (G <= 16) {
+    const auto h = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(h[0]) + __uint_as_float(h[1]);
+  }
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
 // N sums over `waves` neighbouring waves at once, the same in each of their threads, in an order that does not depend
@@ -277,7 +300,7 @@ __device__ __forceinline__ float activate_one(float u, int act) {
 // One pass over the data: a row lies in the registers of its G lanes (or of the block's threads) from the load to the
 // store, so the variance is taken around the mean and not from the sum of squares.  A thread keeps its columns from
 // row to row, and with them gamma and beta.
-template <typename T, int G, int NV>
+template <typename T, int G, int NV, int MODE>
 __global__ __launch_bounds__(G ? kThreads : 64 * kMaxWaves) void layer_norm_fwd_kernel(
     const T* x, int64_t xs, int64_t rows, int cols, const float* __restrict__ gamma, const float* __restrict__ beta,
     float eps, int act, T* y, int64_t ys, float* __restrict__ stats) {
@@ -287,7 +310,7 @@ __global__ __launch_bounds__(G ? kThreads : 64 * kMaxWaves) void layer_norm_fwd_
   const int lane = G ? (int)threadIdx.x & (G - 1) : (int)threadIdx.x;
   const int64_t at_once = G ? kThreads / (G ? G : 1) : 1;
   const Pieces<T, NV> at(lane * V, per_row * V, cols);
-  const bool tiny = cols < V;
+  const bool tiny = G == 8 && cols < V;
   const float n = (float)cols;
   float g[NV][V], b[NV][V];
   load_weights<T, NV>(gamma, at, tiny, g);
@@ -296,7 +319,7 @@ __global__ __launch_bounds__(G ? kThreads : 64 * kMaxWaves) void layer_norm_fwd_
   // (every lane of a wave takes part in the sums: a group past the last row works on that one and stores nothing)
   const int64_t first = blockIdx.x * at_once + (G ? (int64_t)threadIdx.x / (G ? G : 1) : 0);
   u32x4 raw[NV];
-  load_row<T, NV>(x + (first < rows ? first : rows - 1) * xs, at, tiny, raw);
+  load_row<MODE, T, NV>(x + (first < rows ? first : rows - 1) * xs, at, tiny, raw);
   int64_t r = first;
   for (int64_t r0 = blockIdx.x * at_once; r0 < rows; r0 += stride, r += stride) {
     float v[NV][V], s[1] = {0.f};
@@ -306,7 +329,7 @@ __global__ __launch_bounds__(G ? kThreads : 64 * kMaxWaves) void layer_norm_fwd_
       mask(v[k], at.skip[k]);
     }
     if (r0 + stride < rows)  // the next row is under way while this one is worked on
-      load_row<T, NV>(x + (r + stride < rows ? r + stride : rows - 1) * xs, at, tiny, raw);
+      load_row<MODE, T, NV>(x + (r + stride < rows ? r + stride : rows - 1) * xs, at, tiny, raw);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -331,7 +354,7 @@ __global__ __launch_bounds__(G ? kThreads : 64 * kMaxWaves) void layer_norm_fwd_
     if (r < rows) {
 #pragma unroll
       for (int k = 0; k < NV; ++k)
-        if (at.skip[k] < V) store_piece<T, V>(y + r * ys + at.c[k], at.skip[k], v[k]);
+        if (at.skip[k] < V) store_piece<MODE, T, V>(y + r * ys + at.c[k], at.skip[k], v[k]);
       if (stats && lane == 0) {
         stats[r] = mean;
         stats[rows + r] = rstd;
@@ -377,7 +400,7 @@ __global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(const T* x, i
 // dbeta along in registers.  A block works on blockDim / (lanes of a row) rows at once; at the end it adds up what its
 // row groups hold (pairwise, through LDS) and leaves one partial sum per column in part[0 or 1][block][column].
 // `waves`: of a row, for G = 0.  Dynamic LDS: blockDim / 2 * NV * V * 2 floats.
-template <typename T, int G, int NV>
+template <typename T, int G, int NV, int MODE>
 __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
     const T* x, int64_t xs, const T* dy, int64_t dys, int64_t rows, int cols, const float* __restrict__ gamma,
     const float* __restrict__ beta, const float* __restrict__ stats, int act, T* dx, int64_t dxs,
@@ -389,7 +412,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
   const int group = (int)threadIdx.x / per_row, lane = (int)threadIdx.x - group * per_row;
   const int64_t at_once = (int)blockDim.x / per_row;
   const Pieces<T, NV> at(lane * V, per_row * V, cols);
-  const bool tiny = cols < V;
+  const bool tiny = G == 8 && cols < V;
   const float n = (float)cols;
   float g[NV][V], b[NV][V], sg[NV][V], sb[NV][V];
   load_weights<T, NV>(gamma, at, tiny, g);
@@ -403,8 +426,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
   float mean_n, rstd_n;
   const auto fetch = [&](int64_t row) {
     row = row < rows ? row : rows - 1;
-    load_row<T, NV>(x + row * xs, at, tiny, xn);
-    load_row<T, NV>(dy + row * dys, at, tiny, dn);
+    load_row<MODE, T, NV>(x + row * xs, at, tiny, xn);
+    load_row<MODE, T, NV>(dy + row * dys, at, tiny, dn);
     mean_n = stats[row];
     rstd_n = stats[rows + row];
   };
@@ -413,16 +436,16 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
   int turn = 0;
   for (int64_t r0 = blockIdx.x * at_once; r0 < rows; r0 += stride, r += stride, turn ^= 1) {
     const float mean = mean_n, rstd = rstd_n;
+    const bool live = r < rows;
     u32x4 xw[NV];
     float xh[NV][V], t[NV][V], s[2] = {0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       xw[k] = xn[k];
       unpack<T>(dn[k], t[k]);
-      mask(t[k], at.skip[k]);  // with dy = 0 they add nothing to any sum
+      mask(t[k], live ? at.skip[k] : V);  // with dy = 0 they add nothing to any sum
     }
     if (r0 + stride < rows) fetch(r + stride);  // the next row is under way while this one is worked on
-    const bool live = r < rows;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       unpack<T>(xw[k], xh[k]);
@@ -434,13 +457,11 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
     for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (live) {
-          sg[k][j] += t[k][j] * xh[k][j];
-          sb[k][j] += t[k][j];
-        }
+        sg[k][j] = fmaf(t[k][j], xh[k][j], sg[k][j]);
+        sb[k][j] += t[k][j];
         t[k][j] *= g[k][j];
         s[0] += t[k][j];
-        s[1] += t[k][j] * xh[k][j];
+        s[1] = fmaf(t[k][j], xh[k][j], s[1]);
       }
     row_sum<G>(s, waves, sh[turn]);
     const float ma = s[0] / n, mq = s[1] / n;
@@ -448,16 +469,28 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) t[k][j] = rstd * (t[k][j] - ma - xh[k][j] * mq);
-        if (at.skip[k] < V) store_piece<T, V>(dx + r * dxs + at.c[k], at.skip[k], t[k]);
+        for (int j = 0; j < V; ++j) t[k][j] = rstd * fmaf(-mq, xh[k][j], t[k][j] - ma);
+        if (at.skip[k] < V) store_piece<MODE, T, V>(dx + r * dxs + at.c[k], at.skip[k], t[k]);
       }
     }
   }
-  // the upper half of the groups hands its sums to the lower one, until one is left
-  for (int groups = (int)at_once; groups > 1;) {
+  // the groups of a wave first; then the upper half of the waves (G = 0: of the groups) hands its sums to the lower
+  // one, until one is left
+  if constexpr (G != 0 && G < 64) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        sg[k][j] = groups_sum<G>(sg[k][j]);
+        sb[k][j] = groups_sum<G>(sb[k][j]);
+      }
+  }
+  const bool holder = G == 0 || (int)(threadIdx.x & 63) < G;
+  const int number = G ? (int)threadIdx.x >> 6 : group;
+  for (int groups = G ? (int)blockDim.x >> 6 : (int)at_once; groups > 1;) {
     const int half = (groups + 1) / 2;
-    const bool give = group >= half && group < groups, take = group < groups - half;
-    float* slot = acc + (give ? group - half : group) * (NV * V * 2) * per_row + lane;
+    const bool give = holder && number >= half && number < groups, take = holder && number < groups - half;
+    float* slot = acc + (give ? number - half : number) * (NV * V * 2) * per_row + lane;
     if (give)
 #pragma unroll
       for (int k = 0; k < NV; ++k)
@@ -478,14 +511,14 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
     __syncthreads();
     groups = half;
   }
-  if (group == 0) {
+  if (holder && number == 0) {
     float* pg = part + (int64_t)blockIdx.x * cols;
     float* pb = part + (int64_t)(gridDim.x + blockIdx.x) * cols;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
       if (at.skip[k] < V) {
-        store_piece<float, V>(pg + at.c[k], at.skip[k], sg[k]);
-        store_piece<float, V>(pb + at.c[k], at.skip[k], sb[k]);
+        store_piece<kPlain, float, V>(pg + at.c[k], at.skip[k], sg[k]);
+        store_piece<kPlain, float, V>(pb + at.c[k], at.skip[k], sb[k]);
       }
   }
 }
@@ -553,7 +586,7 @@ __global__ __launch_bounds__(kFinish* kFinish) void layer_norm_bwd_finish_kernel
   const float* p = part + (int64_t)blockIdx.y * parts * cols;
   float s = 0.f;
   if (c < cols) {
-#pragma unroll 4
+#pragma unroll 8
     for (int k = slice; k < parts; k += kFinish) s += p[(int64_t)k * cols + c];
   }
   sh[slice][threadIdx.x] = s;
@@ -590,6 +623,8 @@ Shape shape_of(int cols, int vec, int wave) {
   return {0, 0, kMaxWaves};
 }
 
+bool streams(int64_t rows, int cols, int passes, size_t size) { return (double)rows * cols * passes * size > 256e6; }
+
 // blocks that are all on the chip at once (`waves` to each, `room` of them to a SIMD) and have as many turns each
 int64_t blocks_of(int64_t turns, int waves, int room) {
   const int64_t resident = (int64_t)kCus * (4 * room / waves);
@@ -605,8 +640,8 @@ bool extent_ok(int64_t rows, int64_t stride, int cols) {
   return rows >= 0 && cols > 0 && stride >= cols && rows <= (INT64_MAX / 8) / stride;
 }
 
-template <typename T>
-void fwd(const void* x, int64_t xs, int64_t rows, int cols, const float* gamma, const float* beta, float eps, int act,
+template <typename T, int MODE>
+void fwd_as(const void* x, int64_t xs, int64_t rows, int cols, const float* gamma, const float* beta, float eps, int act,
          void* y, int64_t ys, float* stats, hipStream_t st) {
   // 16 elements a thread
   constexpr int kWave = 16 / kVec<T>;
@@ -614,11 +649,11 @@ void fwd(const void* x, int64_t xs, int64_t rows, int cols, const float* gamma, 
   const dim3 block(s.group ? kThreads : 64 * s.waves);
   const int64_t turns = s.group ? ceil_div(rows, kThreads / s.group) : rows;
   const dim3 grid((unsigned)blocks_of(turns, (int)block.x / 64, s.pieces * kVec<T> > 8 ? 4 : s.pieces ? 7 : 8));
-#define CASE(G, NV)                                                                                               \
-  if (s.group == G && s.pieces == NV) {                                                                           \
-    XDFM_LAUNCH("layer_norm_fwd_kernel", st, (layer_norm_fwd_kernel<T, G, NV>), grid, block, 0, (const T*)x, xs,  \
-                rows, cols, gamma, beta, eps, act, (T*)y, ys, stats);                                             \
-    return;                                                                                                       \
+#define CASE(G, NV)                                                                                              \
+  if (s.group == G && s.pieces == NV) {                                                                          \
+    XDFM_LAUNCH("layer_norm_fwd_kernel", st, (layer_norm_fwd_kernel<T, G, NV, MODE>), grid, block, 0, (const T*)x, \
+                xs, rows, cols, gamma, beta, eps, act, (T*)y, ys, stats);                                        \
+    return;                                                                                                      \
   }
   CASE(8, 1) CASE(16, 1) CASE(32, 1) CASE(64, 1) CASE(64, 2)
   if constexpr (kWave == 4) {
@@ -636,8 +671,8 @@ void fwd(const void* x, int64_t xs, int64_t rows, int cols, const float* gamma, 
 constexpr int kBwdWaves = kMaxWaves;
 
 // the number of partial sums that lie in ws afterwards
-template <typename T>
-int bwd(const void* x, int64_t xs, const void* dy, int64_t dys, int64_t rows, int cols, const float* gamma,
+template <typename T, int MODE>
+int bwd_as(const void* x, int64_t xs, const void* dy, int64_t dys, int64_t rows, int cols, const float* gamma,
         const float* beta, const float* stats, int act, void* dx, int64_t dxs, float* ws, hipStream_t st) {
   // 8 elements a thread: with their weights and the weights' gradients they take 6 registers each
   constexpr int kWave = 8 / kVec<T>;
@@ -648,7 +683,7 @@ int bwd(const void* x, int64_t xs, const void* dy, int64_t dys, int64_t rows, in
   const int64_t blocks = blocks_of(ceil_div(rows, at_once), threads / 64, 4);
 #define CASE(G, NV)                                                                                                \
   if (s.group == G && s.pieces == NV) {                                                                            \
-    XDFM_LAUNCH("layer_norm_bwd_kernel", st, (layer_norm_bwd_kernel<T, G, NV>), dim3((unsigned)blocks),            \
+    XDFM_LAUNCH("layer_norm_bwd_kernel", st, (layer_norm_bwd_kernel<T, G, NV, MODE>), dim3((unsigned)blocks),      \
                 dim3((unsigned)threads), (size_t)threads* NV* kVec<T> * sizeof(float), (const T*)x, xs,            \
                 (const T*)dy, dys, rows, cols, gamma, beta, stats, act, (T*)dx, dxs, ws, s.waves);                 \
     return (int)blocks;                                                                                            \
@@ -669,6 +704,20 @@ int bwd(const void* x, int64_t xs, const void* dy, int64_t dys, int64_t rows, in
               dim3(64 * kMaxWaves), 0, (const T*)x, xs, (const T*)dy, dys, rows, cols, gamma, beta, stats, act, (T*)dx,
               dxs);
   return parts;
+}
+
+template <typename T>
+void fwd(const void* x, int64_t xs, int64_t rows, int cols, const float* gamma, const float* beta, float eps, int act,
+         void* y, int64_t ys, float* stats, hipStream_t st) {
+  (streams(rows, cols, 2, sizeof(T)) ? fwd_as<T, kStream> : fwd_as<T, kPlain>)(x, xs, rows, cols, gamma, beta, eps, act,
+                                                                               y, ys, stats, st);
+}
+
+template <typename T>
+int bwd(const void* x, int64_t xs, const void* dy, int64_t dys, int64_t rows, int cols, const float* gamma,
+        const float* beta, const float* stats, int act, void* dx, int64_t dxs, float* ws, hipStream_t st) {
+  return (streams(rows, cols, 3, sizeof(T)) ? bwd_as<T, kStream> : bwd_as<T, kPlain>)(
+      x, xs, dy, dys, rows, cols, gamma, beta, stats, act, dx, dxs, ws, st);
 }
 
 }  // namespace
