@@ -61,17 +61,17 @@ __device__ __forceinline__ Step step_of(const Args& a) {
   return {a.lr / -expm1f(t * a.log_b1), 1.f / sqrtf(-expm1f(t * a.log_b2)), (uint32_t)t};
 }
 
-__device__ __forceinline__ float grad_of(const void* g, int type, int64_t i) {
-  if (type == XDFM_F32) return ((const float*)g)[i];
-  if (type == XDFM_BF16) return (float)((const __bf16*)g)[i];
-  return (float)((const _Float16*)g)[i];
+// (multiplications and additions are not contracted in this build: m and v are the two products' sum.  Root and
+// reciprocal are the hardware's, good to one unit of the last place; the root takes no denormal numbers.)
+__device__ __forceinline__ float root(float v) {
+  const bool small = v < 0x1p-96f;
+  const float r = __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v);
+  return small ? r * 0x1p-32f : r;
 }
-
-// (multiplications and additions are not contracted in this build: m and v are the two products' sum)
 __device__ __forceinline__ float update(float p, float g, float& m, float& v, const Args& a, const Step& s, float wd) {
   m = m * a.b1 + g * a.omb1;
   v = v * a.b2 + (g * g) * a.omb2;
-  return (p - (a.lr * wd) * p) - s.size * m / (sqrtf(v) * s.inv_root + a.eps);
+  return (p - wd * p) - s.size * m * __builtin_amdgcn_rcpf(fmaf(root(v), s.inv_root, a.eps));
 }
 
 __device__ __forceinline__ uint32_t mix(uint32_t a, uint32_t b) { return (a ^ (a >> 15)) * kMul1 + b; }
@@ -93,21 +93,27 @@ __device__ __forceinline__ int scale_of(uint32_t top) {
   const int e = (int)(top >> 23);
   return e < kScaleMin ? kScaleMin : e;
 }
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) x = max(x, (uint32_t)__shfl_xor((int)x, m));
-  return x;
+// the largest over the 16 lanes that hold a block
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
+  return max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ uint32_t block_max(uint32_t x) {
+  x = dpp_max<0xB1>(x);   // lane ^ 1
+  x = dpp_max<0x4E>(x);   // lane ^ 2
+  x = dpp_max<0x141>(x);  // 7 - lane of 8
+  return dpp_max<0x140>(x);  // 15 - lane of 16
 }
 
 __device__ __forceinline__ uint32_t code_of(float size, int shift, uint32_t r20) {
   return (__float_as_uint(ldexpf(size, shift)) + r20) >> 20;
 }
-__device__ __forceinline__ uint8_t code_m(float x, int s, uint32_t r20) {
-  return (uint8_t)(code_of(fabsf(x), 14 - s, r20) | (__float_as_uint(x) >> 24 & 0x80u));
+__device__ __forceinline__ uint32_t code_m(float x, int s, uint32_t r20) {
+  return code_of(fabsf(x), 14 - s, r20) | (__float_as_uint(x) >> 24 & 0x80u);
 }
-__device__ __forceinline__ uint8_t code_v(float x, int s, uint32_t r20) {
+__device__ __forceinline__ uint32_t code_v(float x, int s, uint32_t r20) {
   const uint32_t c = code_of(x, 30 - s, r20);
-  return (uint8_t)(c ? c : x > 0.f);
+  return c ? c : x > 0.f;
 }
 __device__ __forceinline__ float value_m(uint32_t c, int s) {
   const float x = __uint_as_float((c & 0x7Fu) << 20 | (c & 0x80u) << 24);
@@ -117,54 +123,250 @@ __device__ __forceinline__ float value_v(uint32_t c, int s) {
   return s == 255 ? __uint_as_float(0x7FC00000u) : ldexpf(__uint_as_float(c << 20), s - 30);
 }
 
+// ------------------------------------------------------------------ four elements of a thread
+constexpr int kEach = 4;                               // elements of a piece
+constexpr int kPieces = kChunk / (kThreads * kEach);   // of a thread in a whole chunk
+static_assert(kBlock == 16 * kEach && kPieces * kThreads * kEach == kChunk, "16 lanes hold a block");
+
+// pieces of the tensors at any address of their type
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32_any __attribute__((aligned(1)));
+
+template <typename T>
+struct Four;  // T x 4 as they are loaded
+template <>
+struct Four<float> {
+  f32x4 w;
+};
+template <>
+struct Four<__bf16> {
+  u32x2 w;
+};
+template <>
+struct Four<_Float16> {
+  u32x2 w;
+};
+template <>
+struct Four<uint8_t> {
+  uint32_t w;
+};
+
+// elements i .. i + 3 of p (EDGE: those before n, 0 behind)
+template <bool EDGE, bool STREAM, typename T>
+__device__ __forceinline__ Four<T> get(const T* p, int i, int n) {
+  Four<T> r;
+  if (!EDGE || i + kEach <= n) {
+    if constexpr (sizeof(T) == 4)
+      r.w = STREAM ? __builtin_nontemporal_load((const f32x4_any*)(p + i)) : *(const f32x4_any*)(p + i);
+    else if constexpr (sizeof(T) == 2)
+      r.w = STREAM ? __builtin_nontemporal_load((const u32x2_any*)(p + i)) : *(const u32x2_any*)(p + i);
+    else
+      r.w = STREAM ? __builtin_nontemporal_load((const u32_any*)(p + i)) : *(const u32_any*)(p + i);
+  } else {
+    T e[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) e[j] = i + j < n ? p[i + j] : (T)0;
+    __builtin_memcpy(&r.w, e, sizeof(e));
+  }
+  return r;
+}
+
+template <bool EDGE, bool STREAM, typename T>
+__device__ __forceinline__ void put(T* p, int i, int n, const Four<T>& r) {
+  if (!EDGE || i + kEach <= n) {
+    if constexpr (sizeof(T) == 4) {
+      if (STREAM)
+        __builtin_nontemporal_store(r.w, (f32x4_any*)(p + i));
+      else
+        *(f32x4_any*)(p + i) = r.w;
+    } else if constexpr (sizeof(T) == 2) {
+      *(u32x2_any*)(p + i) = r.w;
+    } else {
+      if (STREAM)
+        __builtin_nontemporal_store(r.w, (u32_any*)(p + i));
+      else
+        *(u32_any*)(p + i) = r.w;
+    }
+  } else {
+    T e[kEach];
+    __builtin_memcpy(e, &r.w, sizeof(e));
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (i + j < n) p[i + j] = e[j];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void as_floats(const Four<T>& r, float (&v)[kEach]) {
+  T e[kEach];
+  __builtin_memcpy(e, &r.w, sizeof(e));
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) v[j] = (float)e[j];
+}
+
+// four codes -> values and back
+__device__ __forceinline__ void decode(uint32_t cm, uint32_t cv, int sm, int sv, float (&m)[kEach], float (&v)[kEach]) {
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    m[j] = value_m(cm >> (8 * j) & 0xFFu, sm);
+    v[j] = value_v(cv >> (8 * j) & 0xFFu, sv);
+  }
+}
+
+// (a whole block's 16 lanes call it; what lies behind a tensor's end is 0 and raises no scale)
+template <bool RANDOM>
+__device__ __forceinline__ void encode(const float (&m)[kEach], const float (&v)[kEach], uint2 key, uint32_t index,
+                                       Four<uint8_t>& cm, Four<uint8_t>& cv, int& sm, int& sv) {
+  uint32_t am = 0, av = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    am = max(am, __float_as_uint(m[j]) & 0x7FFFFFFFu);
+    av = max(av, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+  }
+  sm = scale_of(block_max(am));
+  sv = scale_of(block_max(av));
+  cm.w = cv.w = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    uint32_t rm = 1u << 19, rv = 1u << 19;
+    if (RANDOM) {
+      const uint32_t r = random_bits(key, index + j);
+      rm = ((r & 0xFFFFu) << 4) + 8u;
+      rv = ((r >> 16) << 4) + 8u;
+    }
+    cm.w |= (code_m(m[j], sm, rm) & 0xFFu) << (8 * j);
+    cv.w |= (code_v(v[j], sv, rv) & 0xFFu) << (8 * j);
+  }
+}
+
+// ------------------------------------------------------------------ the step
+// The pieces of a thread are loaded first, all of them, then worked on one by one: with 8 blocks on a CU that keeps
+// the memory busy.  EDGE: a tensor's last chunk.
+template <typename T, int N, bool EDGE, bool STREAM>
+__device__ __forceinline__ void step32(const Chunk& c, const Args& a, const Step& s, int first) {
+  const float wd = a.lr * c.wd;
+  float *m = (float*)c.m, *v = (float*)c.v;
+  Four<float> p4[N], m4[N], v4[N];
+  Four<T> g4[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int i = first + k * kThreads * kEach;
+    p4[k] = get<EDGE, STREAM>(c.p, i, c.count);
+    g4[k] = get<EDGE, STREAM>((const T*)c.g, i, c.count);
+    m4[k] = get<EDGE, STREAM>(m, i, c.count);
+    v4[k] = get<EDGE, STREAM>(v, i, c.count);
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int i = first + k * kThreads * kEach;
+    float g[kEach];
+    as_floats(g4[k], g);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      float mj = m4[k].w[j], vj = v4[k].w[j];
+      p4[k].w[j] = update(p4[k].w[j], g[j], mj, vj, a, s, wd);
+      m4[k].w[j] = mj;
+      v4[k].w[j] = vj;
+    }
+    put<EDGE, STREAM>(c.p, i, c.count, p4[k]);
+    put<EDGE, STREAM>(m, i, c.count, m4[k]);
+    put<EDGE, STREAM>(v, i, c.count, v4[k]);
+  }
+}
+
+template <typename T, int N, bool EDGE, bool STREAM>
+__device__ __forceinline__ void step8(const Chunk& c, const Args& a, const Step& s, int first) {
+  const float wd = a.lr * c.wd;
+  const uint2 key = keys_of(a, s.t, c.tensor, c.start);
+  uint8_t *m = (uint8_t*)c.m, *v = (uint8_t*)c.v;
+  Four<float> p4[N];
+  Four<T> g4[N];
+  Four<uint8_t> m4[N], v4[N];
+  int sm[N], sv[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int i = first + k * kThreads * kEach;
+    p4[k] = get<EDGE, STREAM>(c.p, i, c.count);
+    g4[k] = get<EDGE, STREAM>((const T*)c.g, i, c.count);
+    m4[k] = get<EDGE, STREAM>(m, i, c.count);
+    v4[k] = get<EDGE, STREAM>(v, i, c.count);
+    const bool in = !EDGE || i < c.count;  // (its block lies in the tensor)
+    sm[k] = in ? c.sm[i / kBlock] : 0;
+    sv[k] = in ? c.sv[i / kBlock] : 0;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int i = first + k * kThreads * kEach;
+    float g[kEach], mj[kEach], vj[kEach];
+    as_floats(g4[k], g);
+    decode(m4[k].w, v4[k].w, sm[k], sv[k], mj, vj);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      p4[k].w[j] = update(p4[k].w[j], g[j], mj[j], vj[j], a, s, wd);
+      if (EDGE && i + j >= c.count) mj[j] = vj[j] = 0.f;  // (a block of NaN is NaN behind the end too)
+    }
+    put<EDGE, STREAM>(c.p, i, c.count, p4[k]);
+    encode<true>(mj, vj, key, (uint32_t)(c.start + i), m4[k], v4[k], sm[k], sv[k]);
+    put<EDGE, STREAM>(m, i, c.count, m4[k]);
+    put<EDGE, STREAM>(v, i, c.count, v4[k]);
+    if ((threadIdx.x & 15) == 0 && (!EDGE || i < c.count)) {
+      c.sm[i / kBlock] = (uint8_t)sm[k];
+      c.sv[i / kBlock] = (uint8_t)sv[k];
+    }
+  }
+}
+
+template <typename T, int BITS, bool STREAM>
+__device__ __forceinline__ void step_chunk(const Chunk& c, const Args& a, const Step& s) {
+  const int mine = (int)threadIdx.x * kEach;
+  if (c.count == kChunk) {
+    if constexpr (BITS == 32)
+      step32<T, kPieces, false, STREAM>(c, a, s, mine);
+    else
+      step8<T, kPieces, false, STREAM>(c, a, s, mine);
+  } else {
+    for (int first = 0; first < c.count; first += kThreads * kEach) {
+      if constexpr (BITS == 32)
+        step32<T, 1, true, STREAM>(c, a, s, first + mine);
+      else
+        step8<T, 1, true, STREAM>(c, a, s, first + mine);
+    }
+  }
+}
+
+template <int BITS, bool STREAM>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(const Chunk* __restrict__ chunks, Args a) {
   const Chunk c = chunks[blockIdx.x];
   const Step s = step_of(a);
-  float *m = (float*)c.m, *v = (float*)c.v;
-  for (int i = threadIdx.x; i < c.count; i += kThreads) {
-    float mi = m[i], vi = v[i];
-    c.p[i] = update(c.p[i], grad_of(c.g, c.gtype, i), mi, vi, a, s, c.wd);
-    m[i] = mi;
-    v[i] = vi;
-  }
+  if (c.gtype == XDFM_F32)
+    step_chunk<float, BITS, STREAM>(c, a, s);
+  else if (c.gtype == XDFM_BF16)
+    step_chunk<__bf16, BITS, STREAM>(c, a, s);
+  else
+    step_chunk<_Float16, BITS, STREAM>(c, a, s);
 }
 
-// a wave per block of 64
-__global__ __launch_bounds__(kThreads) void adamw8_kernel(const Chunk* __restrict__ chunks, Args a) {
+__global__ __launch_bounds__(kThreads) void adamw_state_read_kernel(const Chunk* __restrict__ chunks, __bf16* out_m,
+                                                                    __bf16* out_v) {
   const Chunk c = chunks[blockIdx.x];
-  const Step s = step_of(a);
-  const uint2 key = keys_of(a, s.t, c.tensor, c.start);
-  uint8_t *m = (uint8_t*)c.m, *v = (uint8_t*)c.v;
-  for (int i0 = threadIdx.x & ~63; i0 < c.count; i0 += kThreads) {
-    const int b = i0 / kBlock, i = i0 + (threadIdx.x & 63);
-    const bool in = i < c.count;
-    float mi = 0.f, vi = 0.f;
-    if (in) {
-      mi = value_m(m[i], c.sm[b]);
-      vi = value_v(v[i], c.sv[b]);
-      c.p[i] = update(c.p[i], grad_of(c.g, c.gtype, i), mi, vi, a, s, c.wd);
+  for (int i = (int)threadIdx.x * kEach; i < c.count; i += kThreads * kEach) {
+    float m[kEach], v[kEach];
+    decode(get<true, false>((const uint8_t*)c.m, i, c.count).w, get<true, false>((const uint8_t*)c.v, i, c.count).w,
+           c.sm[i / kBlock], c.sv[i / kBlock], m, v);
+    Four<__bf16> m4, v4;
+    __bf16 em[kEach], ev[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      em[j] = (__bf16)m[j];
+      ev[j] = (__bf16)v[j];
     }
-    const int sm = scale_of(wave_max(__float_as_uint(fabsf(mi)))), sv = scale_of(wave_max(__float_as_uint(fabsf(vi))));
-    if (in) {
-      const uint32_t r = random_bits(key, (uint32_t)(c.start + i));
-      m[i] = code_m(mi, sm, ((r & 0xFFFFu) << 4) + 8u);
-      v[i] = code_v(vi, sv, ((r >> 16) << 4) + 8u);
-      if (i == i0) {
-        c.sm[b] = (uint8_t)sm;
-        c.sv[b] = (uint8_t)sv;
-      }
-    }
-  }
-}
-
-__global__ __launch_bounds__(kThreads) void adamw_state_read_kernel(const Chunk* __restrict__ chunks,
-                                                                    __bf16* __restrict__ out_m,
-                                                                    __bf16* __restrict__ out_v) {
-  const Chunk c = chunks[blockIdx.x];
-  const uint8_t *m = (const uint8_t*)c.m, *v = (const uint8_t*)c.v;
-  for (int i = threadIdx.x; i < c.count; i += kThreads) {
-    out_m[c.out + i] = (__bf16)value_m(m[i], c.sm[i / kBlock]);
-    out_v[c.out + i] = (__bf16)value_v(v[i], c.sv[i / kBlock]);
+    __builtin_memcpy(&m4.w, em, sizeof(em));
+    __builtin_memcpy(&v4.w, ev, sizeof(ev));
+    put<true, false>(out_m + c.out, i, c.count, m4);
+    put<true, false>(out_v + c.out, i, c.count, v4);
   }
 }
 
@@ -172,19 +374,19 @@ __global__ __launch_bounds__(kThreads) void adamw_state_write_kernel(const Chunk
                                                                      const float* __restrict__ in_m,
                                                                      const float* __restrict__ in_v) {
   const Chunk c = chunks[blockIdx.x];
-  uint8_t *m = (uint8_t*)c.m, *v = (uint8_t*)c.v;
-  for (int i0 = threadIdx.x & ~63; i0 < c.count; i0 += kThreads) {
-    const int b = i0 / kBlock, i = i0 + (threadIdx.x & 63);
-    const bool in = i < c.count;
-    const float mi = in ? in_m[c.out + i] : 0.f, vi = in ? in_v[c.out + i] : 0.f;
-    const int sm = scale_of(wave_max(__float_as_uint(fabsf(mi)))), sv = scale_of(wave_max(__float_as_uint(fabsf(vi))));
-    if (in) {
-      m[i] = code_m(mi, sm, 1u << 19);
-      v[i] = code_v(vi, sv, 1u << 19);
-      if (i == i0) {
-        c.sm[b] = (uint8_t)sm;
-        c.sv[b] = (uint8_t)sv;
-      }
+  for (int first = 0; first < c.count; first += kThreads * kEach) {
+    const int i = first + (int)threadIdx.x * kEach;
+    float m[kEach], v[kEach];
+    as_floats(get<true, false>(in_m + c.out, i, c.count), m);
+    as_floats(get<true, false>(in_v + c.out, i, c.count), v);
+    Four<uint8_t> m4, v4;
+    int sm, sv;
+    encode<false>(m, v, make_uint2(0, 0), 0, m4, v4, sm, sv);
+    put<true, false>((uint8_t*)c.m, i, c.count, m4);
+    put<true, false>((uint8_t*)c.v, i, c.count, v4);
+    if ((threadIdx.x & 15) == 0 && i < c.count) {
+      c.sm[i / kBlock] = (uint8_t)sm;
+      c.sv[i / kBlock] = (uint8_t)sv;
     }
   }
 }
@@ -337,12 +539,16 @@ extern "C" int xdfm_adamw_step(const void* plan, const xdfm_adamw_plan_info* inf
   }
   a.seed_lo = (uint32_t)args->seed;
   a.seed_hi = (uint32_t)(args->seed >> 32);
-  if (info->state_bits == 32)
-    XDFM_LAUNCH("adamw_kernel", stream, adamw_kernel, dim3((unsigned)info->chunks), dim3(kThreads), 0,
-                (const Chunk*)plan, a);
+  const dim3 grid((unsigned)info->chunks);
+  const bool stream_by = (double)info->elements * (info->state_bits == 32 ? 28 : 16) > 256e6;
+  if (info->state_bits == 32 && stream_by)
+    XDFM_LAUNCH("adamw_kernel", stream, (adamw_kernel<32, true>), grid, dim3(kThreads), 0, (const Chunk*)plan, a);
+  else if (info->state_bits == 32)
+    XDFM_LAUNCH("adamw_kernel", stream, (adamw_kernel<32, false>), grid, dim3(kThreads), 0, (const Chunk*)plan, a);
+  else if (stream_by)
+    XDFM_LAUNCH("adamw8_kernel", stream, (adamw_kernel<8, true>), grid, dim3(kThreads), 0, (const Chunk*)plan, a);
   else
-    XDFM_LAUNCH("adamw8_kernel", stream, adamw8_kernel, dim3((unsigned)info->chunks), dim3(kThreads), 0,
-                (const Chunk*)plan, a);
+    XDFM_LAUNCH("adamw8_kernel", stream, (adamw_kernel<8, false>), grid, dim3(kThreads), 0, (const Chunk*)plan, a);
   XDFM_LAUNCH_CHECK();
   return XDFM_OK;
 }
