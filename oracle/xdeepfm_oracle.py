@@ -37,6 +37,11 @@ def cin_final_len(hp):
     return sum(L - nh for (_, L, nh) in cin_shapes(hp))
 
 
+def layer_norm_on(hp):
+    """enable_LN (no counterpart in the reference): a layer norm behind every product of the DNN tower."""
+    return hp.values().get("enable_LN", False) is True
+
+
 def param_shapes(hp):
     """name -> shape, in creation order of the reference graph."""
     shapes = {"embedding": (hp.FEATURE_COUNT, hp.dim)}  # xDeepFM.py:38-42
@@ -69,6 +74,9 @@ def param_shapes(hp):
                     shapes["bn_dnn_%s_%d" % (part, k)] = (size,)
                 for part in ("mm", "mv"):
                     shapes["bnstat_dnn_%s_%d" % (part, k)] = (size,)
+            if layer_norm_on(hp):
+                for part in ("g", "o"):
+                    shapes["ln_dnn_%s_%d" % (part, k)] = (size,)
             last = size
         shapes["dnn_w_out"] = (last, 1)  # :514-516
         shapes["dnn_b_out"] = (1,)  # :517-522
@@ -82,7 +90,8 @@ def param_groups(hp):
     embed = ["embedding"]
     cross = [n for n in names if n.startswith(("cin_f_", "fcin_"))]  # also :336, :364-365
     # batch-norm variables are created by tf.layers, never appended to a params list: no regulariser
-    layer = [n for n in names if n not in embed and n not in cross and not n.startswith("bn")]
+    # (the layer norm's are treated like them)
+    layer = [n for n in names if n not in embed and n not in cross and not n.startswith(("bn", "ln_"))]
     return embed, layer, cross
 
 
@@ -93,8 +102,8 @@ def init_params(hp, seed=0, dtype=torch.float32):
     gen = torch.Generator().manual_seed(seed)
     params = {}
     for name, shape in param_shapes(hp).items():
-        if name.startswith("bn"):  # gamma = 1, beta = 0, moving mean = 0, moving variance = 1
-            one = name.startswith(("bn_cin_g_", "bn_dnn_g_", "bnstat_cin_mv_", "bnstat_dnn_mv_"))
+        if name.startswith(("bn", "ln_")):  # gamma = 1, beta = 0, moving mean = 0, moving variance = 1
+            one = name.startswith(("ln_dnn_g_", "bn_cin_g_", "bn_dnn_g_", "bnstat_cin_mv_", "bnstat_dnn_mv_"))
             t = torch.ones(shape, dtype=torch.float64) if one else torch.zeros(shape, dtype=torch.float64)
         elif name.endswith("_b") or "_b_" in name:
             t = torch.zeros(shape, dtype=torch.float64)
@@ -313,6 +322,10 @@ def forward(params, batch, hp, embedding_rows=None, dropout_masks=None, training
             h = h @ params["dnn_w_%d" % k] + params["dnn_b_%d" % k]
             if hp.enable_BN is True:  # :497-503
                 h = _batch_norm(h, params, "dnn", k, training, moving_out)
+            if layer_norm_on(hp):
+                mean = h.mean(1, keepdim=True)
+                var = ((h - mean) ** 2).mean(1, keepdim=True)
+                h = (h - mean) / torch.sqrt(var + 1e-5) * params["ln_dnn_g_%d" % k] + params["ln_dnn_o_%d" % k]
             if hp.user_dropout and dropout_masks is not None:
                 # _active_layer (base_model.py:335-336): tf.nn.dropout on the pre-activation.  TF's
                 # random stream is not reproducible: the caller supplies m / keep per layer
@@ -372,7 +385,7 @@ def regular_loss(params, hp):
 
 def new_opt_state(params, hp):
     st = {"step": 0}
-    if hp.optimizer == "adam":
+    if hp.optimizer in ("adam", "adamw"):
         st["m"] = {n: torch.zeros_like(p) for n, p in params.items()}
         st["v"] = {n: torch.zeros_like(p) for n, p in params.items()}
         # fp32 beta powers multiplied up step by step, like TF's slot variables
@@ -392,11 +405,21 @@ def new_opt_state(params, hp):
     return st
 
 
-def _apply(name, p, g, st, hp, rows=None):
-    """In-place TF1 update of p (optionally only of p[rows] with g = grad of those rows)."""
+def _apply(name, p, g, st, hp, rows=None, adam_rows=False):
+    """In-place TF1 update of p (optionally only of p[rows] with g = grad of those rows).  adamw: decoupled decay of
+    the matrices, of the table and lin_w by embed_weight_decay; adam_rows: those two take Adam's update instead."""
     lr = hp.learning_rate
     sel = slice(None) if rows is None else rows
-    if hp.optimizer == "adam":
+    of_table = name in ("embedding", "lin_w")
+    if hp.optimizer == "adamw" and not (adam_rows and of_table):
+        m, v, t = st["m"][name], st["v"][name], st["step"]
+        decay = (hp.values().get("embed_weight_decay", 0.0) if of_table else
+                 hp.values().get("weight_decay", 0.01) if p.dim() == 2 else 0.0)
+        m.mul_(0.9).add_(g, alpha=0.1)
+        v.mul_(0.999).add_(g * g, alpha=0.001)
+        p.mul_(1 - lr * decay)
+        p.sub_(lr * (m / (1 - 0.9 ** t)) / ((v / (1 - 0.999 ** t)).sqrt() + 1e-8))
+    elif hp.optimizer in ("adam", "adamw"):
         m, v = st["m"][name], st["v"][name]
         b1, b2, eps = 0.9, 0.999, 1e-8
         if p.dtype == torch.float32:
@@ -441,7 +464,7 @@ def _apply(name, p, g, st, hp, rows=None):
         p[sel] = p[sel] - g * lr
 
 
-def train_step(params, st, batch, hp, mode="dense_exact", dropout_masks=None):
+def train_step(params, st, batch, hp, mode="dense_exact", dropout_masks=None, adam_rows=False):
     """One `sess.run(update)` (base_model.py:367-388): returns (loss, data_loss, grads).
 
     dense_exact : reference semantics -- every variable (the whole table included) takes an
@@ -452,7 +475,7 @@ def train_step(params, st, batch, hp, mode="dense_exact", dropout_masks=None):
     """
     labels = torch.as_tensor(np.asarray(batch["labels"])).to(params["embedding"].dtype)
     st["step"] += 1
-    if hp.optimizer == "adam":
+    if hp.optimizer in ("adam", "adamw"):
         st["b1p"] = np.float32(st["b1p"] * np.float32(0.9))
         st["b2p"] = np.float32(st["b2p"] * np.float32(0.999))
 
@@ -510,7 +533,7 @@ def train_step(params, st, batch, hp, mode="dense_exact", dropout_masks=None):
             if sparse and n in ("embedding", "lin_w"):
                 _apply(n, params[n], g, st, hp, rows=uniq)
             else:
-                _apply(n, params[n], g, st, hp)
+                _apply(n, params[n], g, st, hp, adam_rows=adam_rows)
     for n, t in moving.items():
         params[n].copy_(t)
     return float(loss.detach()), float(dl.detach()), grads, aux
@@ -520,7 +543,7 @@ def _regular_loss_subset(params, hp):
     """regular_loss over the dense parameters only (sparse_rows mode)."""
     total = 0
     for n, p in params.items():
-        if n.startswith("bn"):
+        if n.startswith(("bn", "ln_")):
             continue
         if n.startswith(("cin_f_", "fcin_")):
             total = total + hp.cross_l1 * p.abs().sum() + hp.cross_l2 * torch.sqrt((p**2).sum())

@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 64;  // elements that share a scale
-constexpr int kChunk = 4096;
+constexpr int kChunk = 2048;  // elements: 40 bytes of record for 32 KB of a 16-byte element
 constexpr int kScaleMin = 48;  // units stay normal floats: 2^(48 - 159)
 constexpr uint32_t kMul1 = 0x9E3779B1u;  // 2^32 / golden ratio
 constexpr uint32_t kMul2 = 0x6A09E667u;  // the fraction of sqrt(2)
@@ -133,6 +133,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
 
 template <typename T>
@@ -349,25 +351,64 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Chunk* __restrict
     step_chunk<_Float16, BITS, STREAM>(c, a, s);
 }
 
+// eight elements a thread: 16 bytes of each output
+template <bool EDGE, int N>
+__device__ __forceinline__ void read_pieces(const Chunk& c, __bf16* out_m, __bf16* out_v, int first) {
+  constexpr int kStep = 2 * kThreads * kEach;
+  Four<uint8_t> m4[N][2], v4[N][2];
+  int sm[N], sv[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int i = first + k * kStep;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      m4[k][h] = get<EDGE, false>((const uint8_t*)c.m, i + h * kEach, c.count);
+      v4[k][h] = get<EDGE, false>((const uint8_t*)c.v, i + h * kEach, c.count);
+    }
+    sm[k] = c.sm[i / kBlock];
+    sv[k] = c.sv[i / kBlock];
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int i = first + k * kStep;
+    __bf16 em[2 * kEach], ev[2 * kEach];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float m[kEach], v[kEach];
+      decode(m4[k][h].w, v4[k][h].w, sm[k], sv[k], m, v);
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        em[h * kEach + j] = (__bf16)m[j];
+        ev[h * kEach + j] = (__bf16)v[j];
+      }
+    }
+    if (!EDGE || i + 2 * kEach <= c.count) {
+      u32x4 wm, wv;
+      __builtin_memcpy(&wm, em, sizeof(em));
+      __builtin_memcpy(&wv, ev, sizeof(ev));
+      *(u32x4_any*)(out_m + i) = wm;
+      *(u32x4_any*)(out_v + i) = wv;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2 * kEach; ++j)
+        if (i + j < c.count) {
+          out_m[i + j] = em[j];
+          out_v[i + j] = ev[j];
+        }
+    }
+  }
+}
+
 __global__ __launch_bounds__(kThreads) void adamw_state_read_kernel(const Chunk* __restrict__ chunks, __bf16* out_m,
                                                                     __bf16* out_v) {
   const Chunk c = chunks[blockIdx.x];
-  for (int i = (int)threadIdx.x * kEach; i < c.count; i += kThreads * kEach) {
-    float m[kEach], v[kEach];
-    decode(get<true, false>((const uint8_t*)c.m, i, c.count).w, get<true, false>((const uint8_t*)c.v, i, c.count).w,
-           c.sm[i / kBlock], c.sv[i / kBlock], m, v);
-    Four<__bf16> m4, v4;
-    __bf16 em[kEach], ev[kEach];
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      em[j] = (__bf16)m[j];
-      ev[j] = (__bf16)v[j];
-    }
-    __builtin_memcpy(&m4.w, em, sizeof(em));
-    __builtin_memcpy(&v4.w, ev, sizeof(ev));
-    put<true, false>(out_m + c.out, i, c.count, m4);
-    put<true, false>(out_v + c.out, i, c.count, v4);
-  }
+  const int mine = (int)threadIdx.x * 2 * kEach;
+  out_m += c.out;
+  out_v += c.out;
+  if (c.count == kChunk)
+    read_pieces<false, kPieces / 2>(c, out_m, out_v, mine);
+  else
+    for (int i = mine; i < c.count; i += 2 * kThreads * kEach) read_pieces<true, 1>(c, out_m, out_v, i);
 }
 
 __global__ __launch_bounds__(kThreads) void adamw_state_write_kernel(const Chunk* __restrict__ chunks,

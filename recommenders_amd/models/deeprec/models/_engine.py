@@ -16,6 +16,7 @@ import numpy as np
 import torch
 
 from recommenders_amd import _lib
+from recommenders_amd.models.deeprec.models.adamw import AdamW
 
 _ACT = {"identity": 0, "relu": 1, "sigmoid": 2, "tanh": 3, "elu": 4, "softmax": 5}
 _SOFTMAX = 5  # engine-level code: the kernels get the identity and xdfm_softmax_fwd/bwd follow
@@ -23,7 +24,8 @@ _LOSS = {"log_loss": 0, "cross_entropy_loss": 1, "square_loss": 2}
 # base_model.py:283-302.  ProximalAdagrad / ProximalGradientDescent are built with l1 = l2 = 0
 # there, which makes their updates Adagrad's / plain gradient descent's.
 _OPT = {"sgd": 0, "gd": 0, "pgd": 0, "adam": 1, "adagrad": 2, "padagrad": 2, "rmsprop": 3, "adadelta": 4,
-        "ftrl": 5}
+        "ftrl": 5,
+        "adamw": 1}  # (AdamW for the dense variables; the rows of a sparse table take Adam's row update)
 # (beta1, beta2, eps) as TF1 builds each optimizer from `lr` alone
 _OPT_CONST = {0: (0.0, 0.0, 0.0), 1: (0.9, 0.999, 1e-8), 2: (0.0, 0.0, 0.0), 3: (0.0, 0.9, 1e-10),
               4: (0.0, 0.95, 1e-8), 5: (0.0, 0.0, 0.0)}
@@ -54,6 +56,12 @@ def cin_shapes(hp):
 
 
 BN_MOMENTUM, BN_EPS = 0.95, 0.0001  # xDeepFM.py:237-238, :397-398, :500-501
+LN_EPS = 1e-5
+
+
+def layer_norm_on(hp):
+    """enable_LN (no counterpart in the reference): a layer norm behind every product of the DNN tower."""
+    return hp.values().get("enable_LN", False) is True
 
 
 def bn_state_shapes(hp):
@@ -97,6 +105,9 @@ def dense_param_shapes(hp):
             if hp.enable_BN is True:  # xDeepFM.py:498-503
                 shapes["bn_dnn_g_%d" % k] = (int(size),)
                 shapes["bn_dnn_o_%d" % k] = (int(size),)
+            if layer_norm_on(hp):
+                shapes["ln_dnn_g_%d" % k] = (int(size),)
+                shapes["ln_dnn_o_%d" % k] = (int(size),)
             last = int(size)
         shapes["dnn_w_out"] = (last, 1)
         shapes["dnn_b_out"] = (1,)
@@ -130,12 +141,16 @@ class XDeepFMEngine(object):
         self.F, self.D = int(hp.FIELD_COUNT), int(hp.dim)
         self.fast_d = int(hp.fast_CIN_d) if hp.fast_CIN_d > 0 else 0
         self.use_bn = hp.enable_BN is True
+        self.use_ln = layer_norm_on(hp) and bool(hp.use_DNN_part)
+        if self.use_bn and layer_norm_on(hp):
+            raise ValueError("enable_BN and enable_LN exclude each other")
         self._training = False  # batch statistics (train) or moving statistics (eval / infer)
         # dropout of the DNN layers (base_model.py:335-336): keep = 1 - hparams.dropout[k] in training
         self.use_dropout = bool(hp.user_dropout and hp.use_DNN_part)
         if self.use_dropout and len(hp.dropout) < len(hp.layer_sizes):
             raise ValueError("dropout needs one rate per DNN layer")
         self.dropout_seed = 0x5DEECE66D ^ (0 if seed is None else int(seed))
+        self.round_seed = 0 if seed is None else int(seed)  # of the rounding of 8-bit optimizer states
         self._dropout_live = False  # set by a training forward pass, read by the backward pass
         self.cross_act = 0
         self.cross_path = False
@@ -182,6 +197,7 @@ class XDeepFMEngine(object):
             raise ValueError("embedding_update must be dense_exact, sparse_rows or sparse_lazy")
         self.embedding_update = embedding_update
         self.sparse = embedding_update != "dense_exact"
+        self._adamw_settings(hp)
         self.opt_kind = _OPT.get(hp.optimizer)
         if self.opt_kind is None:
             self.opt_kind = 0  # unknown names fall back to SGD (base_model.py:301-302)
@@ -266,11 +282,13 @@ class XDeepFMEngine(object):
         def slot(like, on, value=0.0):
             return torch.full_like(like, value) if on else None
 
+        coded = self.adamw and self.adamw_bits == 8  # the dense states live as codes in the AdamW objects
         if not self.interleaved:
-            self.table_m, self.table_v = slot(self.table, need_m, m0), slot(self.table, need_v)
-            self.lin_m = slot(self.lin_w, need_m, m0) if self.lin_w is not None else None
-            self.lin_v = slot(self.lin_w, need_v) if self.lin_w is not None else None
-        self.dense_m, self.dense_v = slot(self.dense, need_m, m0), slot(self.dense, need_v)
+            table_m, table_v = need_m and not (coded and not self.sparse), need_v and not (coded and not self.sparse)
+            self.table_m, self.table_v = slot(self.table, table_m, m0), slot(self.table, table_v)
+            self.lin_m = slot(self.lin_w, table_m, m0) if self.lin_w is not None else None
+            self.lin_v = slot(self.lin_w, table_v) if self.lin_w is not None else None
+        self.dense_m, self.dense_v = slot(self.dense, need_m and not coded, m0), slot(self.dense, need_v and not coded)
         self.step = 0
         self.b1p = np.float32(1.0)
         self.b2p = np.float32(1.0)
@@ -290,6 +308,7 @@ class XDeepFMEngine(object):
             self.grad_lin = torch.zeros_like(self.lin_w) if self.lin_w is not None else None
         else:
             self.grad_table = self.grad_lin = None
+        self._make_adamw()
         # segment tables for xdfm_dense_update (host arrays)
         self._seg = self._segment_tables()
         self.err_flag = torch.zeros((1,), dtype=torch.int32, device=dev)
@@ -311,7 +330,7 @@ class XDeepFMEngine(object):
         # stream beside the CIN (matrix-core bound): the two share nothing but emb_out and d_emb
         # regularisation loss (a function of the parameters alone) beside the forward pass
         self.early_reg = (self.overlap_dnn_wanted(hp) and self.sparse and not hp.is_clip_norm
-                          and 0 < len(self.dense_shapes) <= 32)
+                          and 0 < len(self.dense_shapes) <= 32 and not self.adamw)
         self.prepack = os.environ.get("XDFM_CIN_PREPACK", "1") != "0"
         # pooled channels summed over d first (S = sum_d x0*xk, pooled = S Wp): 1/D of their MACs, but
         # measured slower on configs[2] (0.629 against 0.572 ms/step: the layer kernels do not shrink
@@ -392,7 +411,7 @@ class XDeepFMEngine(object):
         if self.lin_w is not None:
             draw(self.lin_w, (self.N, 1))
         for name, shape in self.dense_shapes.items():
-            if name.startswith("bn_"):
+            if name.startswith(("bn_", "ln_")):
                 self.views[name].fill_(1.0 if "_g_" in name else 0.0)  # gamma = 1, beta = 0
             elif name.endswith("_b") or "_b_" in name:
                 self.views[name].zero_()
@@ -418,7 +437,101 @@ class XDeepFMEngine(object):
             if t is not None:
                 # (the dense slots without the alignment filler of the bf16 path: one layout for every engine)
                 sd[key] = self._dense_compact(t) if key.startswith("slot/dense_") else t
+        for where, opt in self._coded_adamw():
+            # as they are, for an engine of the same layout, and as values, for every other one
+            for name, parts in self._codes(opt).items():
+                sd["slot8/%s_%s" % (where, name)] = torch.cat([t.reshape(-1) for t in parts])
+            for name, values in zip("mv", opt.read_state()):
+                if where == "dense":
+                    sd["slot/dense_" + name] = values
+                else:
+                    sd["slot/table_" + name] = values[:self.table.numel()].view(self.table.shape)
+                    if self.lin_w is not None:
+                        sd["slot/lin_" + name] = values[self.table.numel():]
         return sd
+
+    # ------------------------------------------------------------------ AdamW
+    def _adamw_settings(self, hp):
+        """optimizer="adamw" (no counterpart in the reference): its hyper-parameters, and what it excludes."""
+        values = hp.values()
+        self.adamw = hp.optimizer == "adamw"
+        self.weight_decay = float(values.get("weight_decay", 0.01))
+        self.embed_weight_decay = float(values.get("embed_weight_decay", 0.0))
+        self.adamw_bits = int(values.get("adamw_state_bits", 32))
+        if not self.adamw:
+            return
+        if self.adamw_bits not in (32, 8):
+            raise ValueError("adamw_state_bits must be 32 or 8")
+        if self.sparse and self.embed_weight_decay != 0.0:
+            raise ValueError("embed_weight_decay moves every row every step: it needs embedding_update dense_exact")
+        if any(getattr(hp, k) != 0.0 for k in ("embed_l2", "embed_l1", "layer_l2", "layer_l1", "cross_l2", "cross_l1")):
+            raise ValueError("adamw decays the weights by weight_decay / embed_weight_decay: the l1 and l2 terms of "
+                             "the loss must be 0")
+        if hp.is_clip_norm:
+            raise ValueError("adamw does not clip gradients")
+
+    def _make_adamw(self):
+        """The AdamW objects: of the dense variables (one tensor each: matrices decay, vectors do not), and of the
+        table and the linear weights where they are updated densely."""
+        self._adamw_dense = self._adamw_table = None
+        if not self.adamw:
+            return
+
+        def make(params, grads, decay, m, v):
+            slots = dict(slot_m=m, slot_v=v) if self.adamw_bits == 32 else {}
+            return AdamW(params, grads, weight_decay=decay, state_bits=self.adamw_bits, **slots)
+
+        def split(flat):
+            if flat is None:
+                return None
+            return [flat[self.dense_off[i]:self.dense_off[i] + n] for i, n in enumerate(self._dense_sizes)]
+
+        if self.dense_shapes:
+            decay = [self.weight_decay if len(shape) == 2 else 0.0 for shape in self.dense_shapes.values()]
+            self._adamw_dense = make(split(self.dense), split(self.dense_grad), decay, split(self.dense_m),
+                                     split(self.dense_v))
+        if not self.sparse:
+            keep = self.lin_w is not None
+            self._adamw_table = make([self.table] + ([self.lin_w] if keep else []),
+                                     [self.grad_table] + ([self.grad_lin] if keep else []), self.embed_weight_decay,
+                                     [self.table_m] + ([self.lin_m] if keep else []),
+                                     [self.table_v] + ([self.lin_v] if keep else []))
+
+    def _adamw_step(self, opt, salt):
+        b1, b2, eps = _OPT_CONST[1]
+        opt.step(lr=float(self.hp.learning_rate), beta1=b1, beta2=b2, eps=eps, opt_state=self.opt_state,
+                 seed=self.round_seed ^ salt)
+
+    def _coded_adamw(self):
+        """(where, AdamW) of the states that are kept in 8 bits."""
+        if not self.adamw or self.adamw_bits != 8:
+            return []
+        return [(where, opt) for where, opt in (("dense", self._adamw_dense), ("table", self._adamw_table))
+                if opt is not None]
+
+    @staticmethod
+    def _codes(opt):
+        return {"m": opt.slot_m, "v": opt.slot_v, "sm": opt.scale_m, "sv": opt.scale_v}
+
+    def _load_codes(self, sd):
+        """8-bit states: from codes of the same layout, or from values."""
+        for where, opt in self._coded_adamw():
+            codes = self._codes(opt)
+            saved = {name: sd.get("slot8/%s_%s" % (where, name)) for name in codes}
+            if all(t is not None and torch.as_tensor(t).numel() == sum(p.numel() for p in codes[name])
+                   for name, t in saved.items()):
+                for name, parts in codes.items():
+                    whole = torch.as_tensor(saved[name]).to(self.device)
+                    for part, t in zip(torch.split(whole, [p.numel() for p in parts]), parts):
+                        t.view(-1).copy_(part)
+                continue
+            names = ["dense"] if where == "dense" else ["table"] + (["lin"] if self.lin_w is not None else [])
+            values = {x: [sd.get("slot/%s_%s" % (n, x)) for n in names] for x in "mv"}
+            if any(t is None for x in "mv" for t in values[x]):
+                continue  # no optimizer state in this dict
+            opt.write_state(*[torch.cat([torch.as_tensor(np.asarray(t) if not torch.is_tensor(t) else t)
+                                         .to(self.device, torch.float32).reshape(-1) for t in values[x]])
+                              for x in "mv"])
 
     def _dense_compact(self, flat):
         offs, sizes = self.dense_off, self._dense_sizes
@@ -468,6 +581,7 @@ class XDeepFMEngine(object):
                     self._dense_expand(t, sd[key])
                 else:
                     put(t, sd[key])
+        self._load_codes(sd)
         if "step" in sd:
             self.step = int(sd["step"])
             self.b1p = np.float32(sd.get("b1p", 0.9 ** self.step))
@@ -524,7 +638,7 @@ class XDeepFMEngine(object):
         l1 = np.zeros(max(n, 1), dtype=np.float32)
         nl2 = np.zeros(max(n, 1), dtype=np.float32)
         for i, name in enumerate(self.dense_shapes):
-            if name.startswith("bn_"):  # tf.layers variables: in no params list, no regulariser
+            if name.startswith(("bn_", "ln_")):  # tf.layers variables: in no params list, no regulariser
                 continue
             if name.startswith(("cin_f_", "fcin_")):  # cross_params (base_model.py:158-166)
                 l1[i] = hp.cross_l1
@@ -694,9 +808,14 @@ class XDeepFMEngine(object):
             for k, size in enumerate(hp.layer_sizes):
                 buf("h_%d" % k, B, int(size))
                 buf("d_h_%d" % k, B, int(size))
-                if self.use_bn:
+                if self.use_bn or self.use_ln:
                     buf("z_%d" % k, B, int(size))
+                if self.use_bn:
                     buf("bn_stats_dnn_%d" % k, 2 * int(size))
+                if self.use_ln:
+                    buf("ln_stats_%d" % k, 2 * B)
+                    _lib.check(self.lib.xdfm_layer_norm_bwd_workspace_floats(B, int(size), ctypes.byref(sz)))
+                    dnn_part_floats = max(dnn_part_floats, sz.value)
                 if self.use_dropout:
                     buf("drop_%d" % k, B, int(size))
                 _lib.check(self.lib.xdfm_dense_bwd_workspace_floats(B, last, int(size), ctypes.byref(sz)))
@@ -1133,6 +1252,23 @@ class XDeepFMEngine(object):
                                  _ptr(self.grad_views["bn_%s_o_%d" % (where, k)]), self._stream())
         )
 
+    def _ln_fwd(self, x, y, k, B, n, act):
+        _lib.check(
+            self.lib.xdfm_layer_norm_fwd(_ptr(x), n, 0, B, n, _ptr(self.views["ln_dnn_g_%d" % k]),
+                                         _ptr(self.views["ln_dnn_o_%d" % k]), LN_EPS, act, _ptr(y), n,
+                                         _ptr(self.ws["ln_stats_%d" % k]), self._stream())
+        )
+
+    def _ln_bwd(self, x, dy, k, B, n, act):
+        """dy <- gradient w.r.t. the layer norm's input (in place); gamma / beta gradients."""
+        _lib.check(
+            self.lib.xdfm_layer_norm_bwd(_ptr(x), n, _ptr(dy), n, 0, B, n, _ptr(self.views["ln_dnn_g_%d" % k]),
+                                         _ptr(self.views["ln_dnn_o_%d" % k]), _ptr(self.ws["ln_stats_%d" % k]), act,
+                                         _ptr(dy), n, _ptr(self.grad_views["ln_dnn_g_%d" % k]),
+                                         _ptr(self.grad_views["ln_dnn_o_%d" % k]), _ptr(self.ws["part_dnn"]),
+                                         self._stream())
+        )
+
     def _pack_filters(self, B, with_grad):
         """One launch packs the filter images of every CIN layer for this step."""
         ws = self.ws
@@ -1187,27 +1323,30 @@ class XDeepFMEngine(object):
             self._done(ev)
             return
         x, K = ws["emb_out"], self.F * self.D
+        norm = self.use_bn or self.use_ln
         for k, size in enumerate(hp.layer_sizes):
             act = _ACT[hp.activation[k]]
             soft = act == _SOFTMAX
             if soft:
                 act = 0
+            out = ws["z_%d" % k] if norm else ws["h_%d" % k]
             if self.bf16 and K >= 32 and int(size) >= 32:
                 _lib.check(
                     lib.xdfm_dense_bf16_fwd(_ptr(x), _ptr(self.views["dnn_w_%d" % k]), _ptr(self.views["dnn_b_%d" % k]),
-                                            B, K, int(size), act, _ptr(ws["h_%d" % k]), _ptr(ws["bf16_ws"]), st)
+                                            B, K, int(size), 0 if norm else act, _ptr(out), _ptr(ws["bf16_ws"]), st)
                 )
-                x, K = ws["h_%d" % k], int(size)
-                continue
-            _lib.check(
-                lib.xdfm_dense_fwd(_ptr(x), _ptr(self.views["dnn_w_%d" % k]),
-                                   _ptr(self.views["dnn_b_%d" % k]), B, K, int(size),
-                                   0 if (self._dropout_live or self.use_bn) else act,
-                                   _ptr(ws["z_%d" % k] if self.use_bn else ws["h_%d" % k]), st)
-            )
-            if self.use_bn:  # xw_plus_b -> batch norm -> (dropout ->) activation
+            else:
+                _lib.check(
+                    lib.xdfm_dense_fwd(_ptr(x), _ptr(self.views["dnn_w_%d" % k]),
+                                       _ptr(self.views["dnn_b_%d" % k]), B, K, int(size),
+                                       0 if (self._dropout_live or norm) else act, _ptr(out), st)
+                )
+            # xw_plus_b -> norm -> (dropout ->) activation
+            if self.use_bn:
                 self._bn_fwd(ws["z_%d" % k], ws["h_%d" % k], "dnn", k, B, int(size), 1,
                              0 if self._dropout_live else act)
+            elif self.use_ln:
+                self._ln_fwd(ws["z_%d" % k], ws["h_%d" % k], k, B, int(size), 0 if self._dropout_live else act)
             if self._dropout_live:
                 _lib.check(
                     lib.xdfm_dropout_act_fwd(_ptr(ws["h_%d" % k]), _ptr(ws["drop_%d" % k]), B, int(size),
@@ -1226,14 +1365,15 @@ class XDeepFMEngine(object):
 
     def _tower_fused(self):
         """The tower runs as one launch per pass (xdfm_tower_fwd / xdfm_tower_bwd_dx) and the step's small
-        weight gradients as one multi-job launch: fp32, no batch norm / dropout / softmax, 1..4 hidden layers,
+        weight gradients as one multi-job launch: fp32, no norm / dropout / softmax, 1..4 hidden layers,
         the first at most 32 wide, the others at most 64."""
         hp = self.hp
         if not hp.use_DNN_part or self.bf16 or os.environ.get("XDFM_TOWER_FUSED", "1") == "0":
             return False
         sizes = [int(v) for v in hp.layer_sizes]
         return bool(1 <= len(sizes) <= 4 and sizes[0] <= 32 and max(sizes) <= 64 and not self.use_dropout
-                    and not self.use_bn and all(_ACT[a] != _SOFTMAX for a in hp.activation[:len(sizes)]))
+                    and not self.use_bn and not self.use_ln
+                    and all(_ACT[a] != _SOFTMAX for a in hp.activation[:len(sizes)]))
 
     def _tower_desc(self):
         """struct xdfm_tower_desc over the current workspace (cached until it is re-allocated)."""
@@ -1286,11 +1426,11 @@ class XDeepFMEngine(object):
         return jobs
 
     def _dnn_plain(self):
-        """No dropout, batch norm or softmax in the tower: its backward splits into an input-gradient
+        """No dropout, norm or softmax in the tower: its backward splits into an input-gradient
         chain and the weight gradients."""
         hp = self.hp
-        return not (self._dropout_live or self.use_bn or any(_ACT[hp.activation[k]] == _SOFTMAX
-                                                              for k in range(len(hp.layer_sizes))))
+        return not (self._dropout_live or self.use_bn or self.use_ln
+                    or any(_ACT[hp.activation[k]] == _SOFTMAX for k in range(len(hp.layer_sizes))))
 
     def _dnn_backward(self, B, first_layer_dx, phase="all", head_jobs=False):
         """Backward of the DNN tower on the current stream.  first_layer_dx: (buffer, accumulate)
@@ -1359,6 +1499,9 @@ class XDeepFMEngine(object):
                 act = 0
             if self.use_bn:
                 self._bn_bwd(ws["z_%d" % k], acts[k + 1], d_acts[k + 1], "dnn", k, B, sizes[k + 1], 1, act)
+                act = 0
+            elif self.use_ln:
+                self._ln_bwd(ws["z_%d" % k], d_acts[k + 1], k, B, sizes[k + 1], act)
                 act = 0
             if self.bf16 and sizes[k] >= 32 and sizes[k + 1] >= 32:
                 _lib.check(
@@ -1776,7 +1919,9 @@ class XDeepFMEngine(object):
         if sparse and self.catchup_on:
             self._rows_stale = True
         first = True  # the first dense_update writes reg_loss, the others accumulate
-        if not sparse:
+        if not sparse and self.adamw:
+            self._adamw_step(self._adamw_table, 0x7AB1E)
+        elif not sparse:
             one = np.asarray([0, self.N * self.D], dtype=np.int64)
             opt = self._opt_args(clip=clip)
             _lib.check(
@@ -1800,6 +1945,7 @@ class XDeepFMEngine(object):
                         None, ctypes.byref(opt), _ptr(self.stats), _ptr(self.reg_loss), 1, st,
                     )
                 )
+        if not sparse:
             _lib.check(
                 lib.xdfm_embed_clear_rows(_ptr(self.grad_table), _ptr(self.grad_lin) if use_lin else None,
                                           self.D, _ptr(batch.sorted_ids), batch.nnz, st)
@@ -1813,7 +1959,9 @@ class XDeepFMEngine(object):
         clip = float(hp.max_grad_norm) if hp.is_clip_norm else 0.0
         ev_upd = self._mark("dense_update")
         n_seg = len(self.dense_shapes)
-        if n_seg:
+        if self.adamw and n_seg:
+            self._adamw_step(self._adamw_dense, 0xDE45E)  # (no regularisation terms: reg_loss is 0)
+        elif n_seg:
             seg = self._seg
             opt = self._opt_args(clip=clip)
             for s0 in range(0, n_seg, 32):

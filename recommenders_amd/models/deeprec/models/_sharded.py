@@ -542,6 +542,8 @@ class ShardedXDeepFMEngine(XDeepFMEngine):
         XDeepFMEngine.__init__(self, hp, device=device, seed=None if seed is None else seed + 7919 * self.rank,
                                embedding_update=embedding_update, table_rows=self.pad_row + 1,
                                compute_dtype=compute_dtype)
+        # replicated parameters take replicated steps: every rank rounds their 8-bit states alike
+        self.round_seed = 0 if seed is None else int(seed)
         # requests of a fixed number of slots per owner: no sizes from the host, the step's exchanges move
         # equally sized messages (XDFM_SHARD_FIXED=0: sized requests, one host synchronisation per step)
         self.fixed = os.environ.get("XDFM_SHARD_FIXED", "1") != "0" and self.exchange.virtual_world == 1
@@ -873,6 +875,12 @@ class ShardedXDeepFMEngine(XDeepFMEngine):
                 ctypes.byref(opt), _ptr(pieces), None, recv_c.stride(0) if use_lin else 0, None, st,
             )
         )
+        if self.adamw:
+            self._adamw_step(self._adamw_table, 0x7AB1E)
+            _lib.check(lib.xdfm_embed_clear_rows(_ptr(self.grad_table), _ptr(self.grad_lin) if use_lin else None, D,
+                                                 _ptr(plan.owner_sorted_ids), n, st))
+            self._done(ev)
+            return
         one = np.asarray([0, self.N * D], dtype=np.int64)
         _lib.check(
             lib.xdfm_dense_update(
@@ -1164,6 +1172,8 @@ class ShardedXDeepFMEngine(XDeepFMEngine):
             if key in sd:
                 t = torch.as_tensor(np.asarray(sd[key]) if not torch.is_tensor(sd[key]) else sd[key])
                 local[key] = t[r::G]
+        for key in [k for k in local if k.startswith("slot8/table_")]:
+            del local[key]  # (codes of blocks that cross rows: this rank's rows come from the values)
         self.load_state(local)
 
     def gather_global_table(self):
