@@ -330,12 +330,10 @@ __device__ __forceinline__ void step_chunk(const Chunk& c, const Args& a, const 
     else
       step8<T, kPieces, false, STREAM>(c, a, s, mine);
   } else {
-    for (int first = 0; first < c.count; first += kThreads * kEach) {
-      if constexpr (BITS == 32)
-        step32<T, 1, true, STREAM>(c, a, s, first + mine);
-      else
-        step8<T, 1, true, STREAM>(c, a, s, first + mine);
-    }
+    if constexpr (BITS == 32)
+      step32<T, kPieces, true, STREAM>(c, a, s, mine);
+    else
+      step8<T, kPieces, true, STREAM>(c, a, s, mine);
   }
 }
 

@@ -290,12 +290,6 @@ __device__ __forceinline__ void through_act(float (&d)[NV][V], const float (&xh)
 #undef XDFM_EACH
 }
 
-__device__ __forceinline__ float activate_one(float u, int act) {
-  float v[1][1] = {{u}};
-  activate_all(v, act);
-  return v[0][0];
-}
-
 // ------------------------------------------------------------------ forward
 // One pass over the data: a row lies in the registers of its G lanes (or of the block's threads) from the load to the
 // store, so the variance is taken around the mean and not from the sum of squares.  A thread keeps its columns from
@@ -363,31 +357,52 @@ __global__ __launch_bounds__(G ? kThreads : 64 * kMaxWaves) void layer_norm_fwd_
   }
 }
 
-// Rows that the registers of a block do not hold: three passes over the row, which its caches serve.
+// Rows that the registers of a block do not hold: three passes over the row, which the caches serve.
 template <typename T>
-__global__ __launch_bounds__(1024) void layer_norm_fwd_long_kernel(const T* x, int64_t xs, int64_t rows, int cols,
-                                                                   const float* __restrict__ gamma,
-                                                                   const float* __restrict__ beta, float eps, int act,
-                                                                   T* y, int64_t ys, float* __restrict__ stats) {
+__global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_fwd_long_kernel(
+    const T* x, int64_t xs, int64_t rows, int cols, const float* __restrict__ gamma, const float* __restrict__ beta,
+    float eps, int act, T* y, int64_t ys, float* __restrict__ stats) {
+  constexpr int V = kVec<T>;
   __shared__ float sh[2][kMaxWaves][1];
-  const int waves = (int)blockDim.x >> 6;
+  const int waves = (int)blockDim.x >> 6, c0 = (int)threadIdx.x * V, step = (int)blockDim.x * V;
   const float n = (float)cols;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T* xr = x + r * xs;
-    T* yr = y + r * ys;
-    float s[1] = {0.f};
-    for (int c = threadIdx.x; c < cols; c += blockDim.x) s[0] += (float)xr[c];
+    const auto piece = [&](int c, float (&v)[1][V]) {
+      const Pieces<T, 1> at(c, 0, cols);
+      u32x4 w[1];
+      load_row<kPlain, T, 1>(x + r * xs, at, false, w);
+      unpack<T>(w[0], v[0]);
+      return at;
+    };
+    float s[1] = {0.f}, q[1] = {0.f}, v[1][V];
+    for (int c = c0; c < cols; c += step) {
+      const Pieces<T, 1> at = piece(c, v);
+      mask(v[0], at.skip[0]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[0] += v[0][j];
+    }
     waves_sum(s, waves, sh[0]);
     const float mean = s[0] / n;
-    float q[1] = {0.f};
-    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
-      const float d = (float)xr[c] - mean;
-      q[0] += d * d;
+    for (int c = c0; c < cols; c += step) {
+      const Pieces<T, 1> at = piece(c, v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[0][j] -= mean;
+      mask(v[0], at.skip[0]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) q[0] = fmaf(v[0][j], v[0][j], q[0]);
     }
     waves_sum(q, waves, sh[1]);
     const float rstd = 1.f / sqrtf(q[0] / n + eps);
-    for (int c = threadIdx.x; c < cols; c += blockDim.x)
-      yr[c] = (T)activate_one(((float)xr[c] - mean) * rstd * gamma[c] + beta[c], act);
+    for (int c = c0; c < cols; c += step) {
+      const Pieces<T, 1> at = piece(c, v);
+      float g[1][V], b[1][V];
+      load_weights<T, 1>(gamma, at, false, g);
+      load_weights<T, 1>(beta, at, false, b);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[0][j] = (v[0][j] - mean) * rstd * g[0][j] + b[0][j];
+      activate_all(v, act);
+      store_piece<kPlain, T, V>(y + r * ys + at.c[0], at.skip[0], v[0]);
+    }
     if (stats && threadIdx.x == 0) {
       stats[r] = mean;
       stats[rows + r] = rstd;
@@ -523,34 +538,60 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
   }
 }
 
+// A piece of a long row: du in t, xhat in xh, and what counts of it.
 template <typename T>
-__global__ __launch_bounds__(1024) void layer_norm_bwd_long_kernel(const T* x, int64_t xs, const T* dy, int64_t dys,
-                                                                   int64_t rows, int cols,
-                                                                   const float* __restrict__ gamma,
-                                                                   const float* __restrict__ beta,
-                                                                   const float* __restrict__ stats, int act, T* dx,
-                                                                   int64_t dxs) {
+struct LongPiece {
+  float g[1][kVec<T>], xh[1][kVec<T>], t[1][kVec<T>];
+  Pieces<T, 1> at;
+  __device__ __forceinline__ LongPiece(const T* x, const T* dy, const float* __restrict__ gamma,
+                                       const float* __restrict__ beta, float mean, float rstd, int act, int c, int cols)
+      : at(c, 0, cols) {
+    u32x4 xw[1], dw[1];
+    float b[1][kVec<T>];
+    load_row<kPlain, T, 1>(x, at, false, xw);
+    load_row<kPlain, T, 1>(dy, at, false, dw);
+    load_weights<T, 1>(gamma, at, false, g);
+    load_weights<T, 1>(beta, at, false, b);
+    unpack<T>(xw[0], xh[0]);
+    unpack<T>(dw[0], t[0]);
+    mask(t[0], at.skip[0]);
+#pragma unroll
+    for (int j = 0; j < kVec<T>; ++j) xh[0][j] = (xh[0][j] - mean) * rstd;
+    through_act<T>(t, xh, xw, g, b, mean, rstd, act);
+  }
+};
+
+// Rows that the registers of a block do not hold: x and dy are read three times, twice here (the second time out of the
+// caches) and once for the weights' gradients.
+template <typename T>
+__global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_long_kernel(
+    const T* x, int64_t xs, const T* dy, int64_t dys, int64_t rows, int cols, const float* __restrict__ gamma,
+    const float* __restrict__ beta, const float* __restrict__ stats, int act, T* dx, int64_t dxs) {
+  constexpr int V = kVec<T>;
   __shared__ float sh[2][kMaxWaves][2];
-  const int waves = (int)blockDim.x >> 6;
+  const int waves = (int)blockDim.x >> 6, c0 = (int)threadIdx.x * V, step = (int)blockDim.x * V;
   const float n = (float)cols;
   int turn = 0;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x, turn ^= 1) {
     const float mean = stats[r], rstd = stats[rows + r];
     float s[2] = {0.f, 0.f};
-    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
-      const float xv = (float)x[r * xs + c], xhat = (xv - mean) * rstd;
-      const float t = (float)dy[r * dys + c] *
-                      slope(xhat * gamma[c] + beta[c], act, xv, mean, rstd, gamma[c], beta[c]) * gamma[c];
-      s[0] += t;
-      s[1] += t * xhat;
+    for (int c = c0; c < cols; c += step) {
+      const LongPiece<T> p(x + r * xs, dy + r * dys, gamma, beta, mean, rstd, act, c, cols);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float t = p.t[0][j] * p.g[0][j];
+        s[0] += t;
+        s[1] = fmaf(t, p.xh[0][j], s[1]);
+      }
     }
     waves_sum(s, waves, sh[turn]);
     const float ma = s[0] / n, mq = s[1] / n;
-    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
-      const float xv = (float)x[r * xs + c], xhat = (xv - mean) * rstd;
-      const float t = (float)dy[r * dys + c] *
-                      slope(xhat * gamma[c] + beta[c], act, xv, mean, rstd, gamma[c], beta[c]) * gamma[c];
-      dx[r * dxs + c] = (T)(rstd * (t - ma - xhat * mq));
+    for (int c = c0; c < cols; c += step) {
+      const LongPiece<T> p(x + r * xs, dy + r * dys, gamma, beta, mean, rstd, act, c, cols);
+      float d[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[j] = rstd * fmaf(-mq, p.xh[0][j], p.t[0][j] * p.g[0][j] - ma);
+      store_piece<kPlain, T, V>(dx + r * dxs + p.at.c[0], p.at.skip[0], d);
     }
   }
 }
@@ -560,19 +601,23 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void layer_norm_bwd_long_sums_kernel(
     const T* x, int64_t xs, const T* dy, int64_t dys, int64_t rows, int cols, const float* __restrict__ gamma,
     const float* __restrict__ beta, const float* __restrict__ stats, int act, int parts, float* __restrict__ part) {
-  const int c = blockIdx.x * kThreads + threadIdx.x, p = blockIdx.y;
+  constexpr int V = kVec<T>;
+  const int c = ((int)blockIdx.x * kThreads + (int)threadIdx.x) * V, p = blockIdx.y;
   if (c >= cols) return;
-  const float g = gamma[c], b = beta[c];
-  float sg = 0.f, sb = 0.f;
+  float sg[V], sb[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) sg[j] = sb[j] = 0.f;
   for (int64_t r = p; r < rows; r += parts) {
-    const float mean = stats[r], rstd = stats[rows + r];
-    const float xv = (float)x[r * xs + c], xhat = (xv - mean) * rstd;
-    const float du = (float)dy[r * dys + c] * slope(xhat * g + b, act, xv, mean, rstd, g, b);
-    sg += du * xhat;
-    sb += du;
+    const LongPiece<T> q(x + r * xs, dy + r * dys, gamma, beta, stats[r], stats[rows + r], act, c, cols);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      sg[j] = fmaf(q.t[0][j], q.xh[0][j], sg[j]);
+      sb[j] += q.t[0][j];
+    }
   }
-  part[(int64_t)p * cols + c] = sg;
-  part[(int64_t)(parts + p) * cols + c] = sb;
+  const Pieces<T, 1> at(c, 0, cols);
+  store_piece<kPlain, float, V>(part + (int64_t)p * cols + at.c[0], at.skip[0], sg);
+  store_piece<kPlain, float, V>(part + (int64_t)(parts + p) * cols + at.c[0], at.skip[0], sb);
 }
 
 // dgamma (blockIdx.y = 0) and dbeta from the blocks' partial sums: 32 columns by 32 slices of the parts per block
@@ -666,8 +711,9 @@ void fwd_as(const void* x, int64_t xs, int64_t rows, int cols, const float* gamm
               cols, gamma, beta, eps, act, (T*)y, ys, stats);
 }
 
-// waves of a backward block, whose row groups share one partial sum: 16 leave 256 partial sums on a full chip (with 4
-// waves a block 1024; 512 columns of bf16 by 16384 rows: 14.6 against 16.6 us, 2496 columns, 5 waves a row: 56 against 108)
+// Waves of a backward block, whose row groups share one partial sum.  16 leave 256 partial sums on a full chip (with 4
+// waves a block 1024; 512 columns of bf16 by 16384 rows: 14.6 against 16.6 us; 2496 columns, 5 waves a row: 56 against
+// 108).  Where that would leave CUs without a block, 8 (20 x 8192 fp32: 7.3 against 8.2 us; 65536 rows: 9.0 and 8.9).
 constexpr int kBwdWaves = kMaxWaves;
 
 // the number of partial sums that lie in ws afterwards
@@ -678,7 +724,8 @@ int bwd_as(const void* x, int64_t xs, const void* dy, int64_t dys, int64_t rows,
   constexpr int kWave = 8 / kVec<T>;
   const Shape s = shape_of(cols, kVec<T>, kWave);
   const int per_row = s.group ? s.group : 64 * s.waves;
-  const int at_once = s.group ? kBwdWaves * 64 / s.group : s.waves < kBwdWaves ? kBwdWaves / s.waves : 1;
+  const int at_most = kBwdWaves * 64 / per_row;
+  const int at_once = s.group && ceil_div(rows, at_most) < kCus ? at_most / 2 : at_most;
   const int threads = at_once * per_row;
   const int64_t blocks = blocks_of(ceil_div(rows, at_once), threads / 64, 4);
 #define CASE(G, NV)                                                                                                \
@@ -696,9 +743,9 @@ int bwd_as(const void* x, int64_t xs, const void* dy, int64_t dys, int64_t rows,
   }
 #undef CASE
   // (the sums first: dx may be dy or x)
-  const int parts = (int)(rows < 64 ? 1 : rows < 16384 ? rows / 64 : 256);
+  const int parts = (int)(rows < 16 ? 1 : rows < 16 * kCus ? rows / 16 : kCus);
   XDFM_LAUNCH("layer_norm_bwd_long_sums_kernel", st, layer_norm_bwd_long_sums_kernel<T>,
-              dim3((unsigned)ceil_div(cols, kThreads), (unsigned)parts), dim3(kThreads), 0, (const T*)x, xs,
+              dim3((unsigned)ceil_div(cols, kThreads * kVec<T>), (unsigned)parts), dim3(kThreads), 0, (const T*)x, xs,
               (const T*)dy, dys, rows, cols, gamma, beta, stats, act, parts, ws);
   XDFM_LAUNCH("layer_norm_bwd_long_kernel", st, layer_norm_bwd_long_kernel<T>, dim3((unsigned)blocks_of(rows, kMaxWaves, 8)),
               dim3(64 * kMaxWaves), 0, (const T*)x, xs, (const T*)dy, dys, rows, cols, gamma, beta, stats, act, (T*)dx,
