@@ -414,7 +414,7 @@ typedef struct xdfm_adamw_plan_info {
 } xdfm_adamw_plan_info;
 
 typedef struct xdfm_adamw_args {
-  double lr, beta1, beta2, eps;
+  double lr, beta1, beta2, eps; /* betas in [0, 1), eps in [1e-30, 1e30] */
   const float* opt_state; /* NULL, or device: t = opt_state[3] (xdfm_opt_advance), so that a step can be captured */
   int64_t step;           /* t, 1 for the first step; used where opt_state is NULL */
   uint64_t seed;          /* of the rounding of 8-bit states */
@@ -783,7 +783,7 @@ int xdfm_bn_bwd_apply(const float* x, const float* y, const float* dy, int64_t B
  * the DNN tower (no counterpart in the reference, which normalises over the batch, xDeepFM.py:497-503).
  *   xhat = (x - mean) * rstd, mean and rstd = 1 / sqrt(var + eps) over the row's `cols` elements (biased
  *   variance);  y = act(gamma * xhat + beta)
- *   x, y, dy, dx: [rows, cols] of `dtype` (XDFM_F32, XDFM_BF16, XDFM_F16), *_stride elements (cols at least)
+ *   x, y, dy, dx: [rows, cols] of `dtype` (XDFM_F32, XDFM_BF16, XDFM_F16), cols <= 2^30, *_stride elements (cols at least)
  *     between consecutive rows, any alignment of the type; what lies between rows is neither read nor
  *     written.  gamma, beta, dgamma, dbeta [cols] and stats are fp32, as is all arithmetic.
  *   stats [2, rows] (NULL ok): mean, then rstd, for the backward pass.

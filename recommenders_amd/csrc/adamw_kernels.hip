@@ -508,8 +508,8 @@ int make_plan(const xdfm_adamw_tensor* t, int n, int bits, Chunk* image, xdfm_ad
       c.gtype = x.grad_dtype;
     }
     out += x.n;
+    XDFM_REQUIRE(chunks < (int64_t)1 << 31, "xdfm_adamw_plan: too many elements");
   }
-  XDFM_REQUIRE(chunks < (int64_t)1 << 31, "xdfm_adamw_plan: too many elements");
   info->bytes = chunks * (int64_t)sizeof(Chunk);
   info->chunks = chunks;
   info->elements = out;
@@ -555,7 +555,7 @@ extern "C" int xdfm_adamw_step(const void* plan, const xdfm_adamw_plan_info* inf
   XDFM_REQUIRE(std::isfinite(args->lr) && args->lr >= 0, "xdfm_adamw_step: lr has to be finite and not negative");
   XDFM_REQUIRE(args->beta1 >= 0 && args->beta1 < 1 && args->beta2 >= 0 && args->beta2 < 1,
                "xdfm_adamw_step: beta1 and beta2 have to lie in [0, 1)");
-  XDFM_REQUIRE(std::isfinite(args->eps) && (float)args->eps > 0.f, "xdfm_adamw_step: eps has to be positive");
+  XDFM_REQUIRE(args->eps >= 1e-30 && args->eps <= 1e30, "xdfm_adamw_step: eps has to lie in [1e-30, 1e30]");
   XDFM_REQUIRE(args->opt_state || args->step >= 1, "xdfm_adamw_step: steps count from 1");
   if (info->chunks == 0) return XDFM_OK;
   Args a;

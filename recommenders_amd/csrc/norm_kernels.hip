@@ -680,9 +680,9 @@ bool act_ok(int act) { return act >= XDFM_ACT_IDENTITY && act <= XDFM_ACT_ELU; }
 bool dtype_ok(int t) { return t == XDFM_F32 || t == XDFM_BF16 || t == XDFM_F16; }
 bool aligned(const void* p, int dtype) { return ((uintptr_t)p & (dtype == XDFM_F32 ? 3 : 1)) == 0; }
 
-// rows * stride elements have to be addressable
+// rows * stride elements have to be addressable, and a column's number plus a block's stride an int
 bool extent_ok(int64_t rows, int64_t stride, int cols) {
-  return rows >= 0 && cols > 0 && stride >= cols && rows <= (INT64_MAX / 8) / stride;
+  return rows >= 0 && cols > 0 && cols <= 1 << 30 && stride >= cols && rows <= (INT64_MAX / 8) / stride;
 }
 
 template <typename T, int MODE>
@@ -794,7 +794,8 @@ extern "C" int xdfm_layer_norm_fwd(const void* x, int64_t x_stride, int32_t dtyp
 }
 
 extern "C" int xdfm_layer_norm_bwd_workspace_floats(int64_t rows, int32_t cols, size_t* floats) {
-  XDFM_REQUIRE(floats && rows >= 0 && cols > 0, "xdfm_layer_norm_bwd_workspace_floats: bad argument");
+  XDFM_REQUIRE(floats && rows >= 0 && cols > 0 && cols <= 1 << 30,
+               "xdfm_layer_norm_bwd_workspace_floats: bad argument");
   *floats = (size_t)2 * (rows < 1 ? 1 : rows < kMaxParts ? rows : kMaxParts) * cols;
   return XDFM_OK;
 }

@@ -76,7 +76,6 @@ class AdamW(object):
         _lib.check(_lib.lib.xdfm_adamw_plan(table, len(params), state_bits, image.data_ptr(), image.numel() * 8,
                                             ctypes.byref(self._info)))
         self._plan = image.to(self.device)  # (a copy from pageable memory: done when this returns)
-        self._args = _lib.AdamWArgs()
         self._index = self._plan.device.index
         self._call = (self._plan.data_ptr(), ctypes.byref(self._info))
         self.elements = int(self._info.elements)
@@ -115,17 +114,15 @@ class AdamW(object):
         in a HIP graph.  ``seed``: of the rounding of 8-bit states."""
         if (step is None) == (opt_state is None):
             raise ValueError("AdamW.step takes either step or opt_state")
-        a = self._args
-        a.lr, a.beta1, a.beta2, a.eps = lr, beta1, beta2, eps
-        a.seed = seed & (2 ** 64 - 1)
         if opt_state is None:
-            a.step, a.opt_state = step, None
+            at = None
         else:
             if (opt_state.dtype != torch.float32 or opt_state.device != self.device or opt_state.numel() < 4
                     or not opt_state.is_contiguous()):
                 raise ValueError("opt_state has to be four contiguous floats on %s" % self.device)
-            a.step, a.opt_state = 0, opt_state.data_ptr()
-        self._enqueue(_lib.lib.xdfm_adamw_step, ctypes.byref(a))
+            step, at = 0, opt_state.data_ptr()
+        args = _lib.AdamWArgs(lr, beta1, beta2, eps, at, step, seed & (2 ** 64 - 1))
+        self._enqueue(_lib.lib.xdfm_adamw_step, ctypes.byref(args))
 
     def _values(self, t, dtype, what):
         if t.dtype != dtype or t.device != self.device or t.numel() != self.elements or not t.is_contiguous():

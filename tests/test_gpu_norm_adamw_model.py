@@ -245,6 +245,80 @@ def test_sharded_engine_takes_the_same_steps():
                 assert d <= (max(2e-4 * float(sa[k].abs().max()), 1e-6) if bits == 32 else 2 * 2 * 1.47 * 0.01), k
 
 
+def _two_rank_worker(rank, world, port, bits, mode, out):
+    """One rank of two processes that share cuda:0 and talk over gloo with host-staged exchanges."""
+    import os
+
+    import torch.distributed as dist
+
+    from oracle import ffm_iterator_oracle as O
+
+    os.environ["MASTER_ADDR"] = "127.0.0.1"
+    os.environ["MASTER_PORT"] = str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        hp = make_hp(enable_LN=True, optimizer="adamw", adamw_state_bits=bits, learning_rate=0.01, FEATURE_COUNT=301,
+                     loss="cross_entropy_loss")
+        p32 = start(hp, 9)
+        eng = ShardedXDeepFMEngine(hp, seed=7, embedding_update=mode)
+        eng.load_global_state({k: v.clone() for k, v in p32.items()})
+        p64 = {k: v.double() for k, v in p32.items()}
+        st = X.new_opt_state(p64, hp)
+        rng = np.random.default_rng(21)  # every rank draws the same global batches
+        per = 48
+        for step in range(4):
+            labels, feats = random_features(rng, per * world, hp.FIELD_COUNT, hp.FEATURE_COUNT)
+            mine = slice(rank * per, (rank + 1) * per)
+            loss, dloss = eng.train_step(upload(eng, O.convert(labels[mine], feats[mine], hp.FIELD_COUNT,
+                                                               hp.FEATURE_COUNT)))
+            tot = torch.stack([loss, dloss]).double().cpu()
+            dist.all_reduce(tot)
+            if bits == 32:
+                o = X.train_step(p64, st, O.convert(labels, feats, hp.FIELD_COUNT, hp.FEATURE_COUNT), hp,
+                                 adam_rows=mode != "dense_exact")
+                close(float(tot[0]), o[0], 2e-5, "loss step %d" % step)
+        eng.check_errors()
+        # the replicated variables and their states: the same bits on every rank
+        flat = [eng.dense.cpu()] + [t.cpu() for n, t in sorted(eng.state_dict().items()) if "/dense_" in n]
+        for t in flat:
+            both = [torch.empty_like(t) for _ in range(world)]
+            dist.all_gather(both, t)
+            assert torch.equal(both[0], both[1])
+        if bits == 32:
+            table, lin = eng.gather_global_table()
+            check_params({**{k: eng.views[k] for k in eng.dense_shapes}, "embedding": table, "lin_w": lin}, p64, 5e-4)
+        out.put((rank, "ok"))
+    except Exception:  # noqa: BLE001
+        import traceback
+
+        out.put((rank, traceback.format_exc()))
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("mode", ["dense_exact", "sparse_rows"])
+def test_two_ranks_stay_together(bits, mode):
+    """World size 2: the norm needs no exchange (its weights' gradients ride in the all-reduce of the dense ones), the
+    replicated variables take the same step on every rank, rounding of 8-bit states included."""
+    import socket
+
+    import torch.multiprocessing as mp
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    out = ctx.Queue()
+    procs = [ctx.Process(target=_two_rank_worker, args=(r, 2, port, bits, mode, out)) for r in range(2)]
+    for p in procs:
+        p.start()
+    res = [out.get(timeout=100) for _ in procs]
+    for p in procs:
+        p.join(timeout=30)
+    assert sorted(res) == [(r, "ok") for r in range(2)], res
+
+
 def test_fit_with_a_norm_and_adamw(tmp_path):
     from recommenders_amd.models.deeprec.io.iterator import FFMTextIterator
     from recommenders_amd.models.deeprec.models.xDeepFM import XDeepFMModel

@@ -33,7 +33,7 @@ def norm_bwd(**kw):
 @pytest.mark.parametrize("kw,text", [
     (dict(dtype=3), "element type"), (dict(dtype=-1), "element type"), (dict(act=5), "activation"),
     (dict(act=-1), "activation"), (dict(rows=-1), "bad sizes"), (dict(cols=0), "bad sizes"), (dict(xs=7), "bad sizes"),
-    (dict(ys=7), "bad sizes"), (dict(rows=1 << 62), "bad sizes"), (dict(eps=0.0), "eps"), (dict(eps=-1.0), "eps"),
+    (dict(ys=7), "bad sizes"), (dict(rows=1 << 62), "bad sizes"), (dict(cols=(1 << 30) + 1, xs=1 << 31, ys=1 << 31), "bad sizes"), (dict(eps=0.0), "eps"), (dict(eps=-1.0), "eps"),
     (dict(eps=float("nan")), "eps"), (dict(x=None), "null"), (dict(y=None), "null"), (dict(gamma=None), "null"),
     (dict(beta=None), "null"), (dict(x=4097), "misaligned"), (dict(y=8194), "misaligned"),
     (dict(dtype=1, x=4097), "misaligned"), (dict(y=4096, ys=9), "same stride"),
@@ -59,6 +59,7 @@ def test_layer_norm_workspace():
     refused(lib.xdfm_layer_norm_bwd_workspace_floats(4, 0, ctypes.byref(size)), "bad argument")
     refused(lib.xdfm_layer_norm_bwd_workspace_floats(-1, 4, ctypes.byref(size)), "bad argument")
     refused(lib.xdfm_layer_norm_bwd_workspace_floats(4, 4, None), "bad argument")
+    refused(lib.xdfm_layer_norm_bwd_workspace_floats(4, (1 << 30) + 1, ctypes.byref(size)), "bad argument")
     assert norm_fwd(rows=0, x=None, y=None) == 0  # no rows: nothing to do
 
 
@@ -140,7 +141,7 @@ def test_adamw_step_refuses():
     nan, inf = float("nan"), float("inf")
     for kw, text in ((dict(lr=-1.0), "lr"), (dict(lr=nan), "lr"), (dict(lr=inf), "lr"), (dict(beta1=1.0), "beta1"),
                      (dict(beta1=-0.1), "beta1"), (dict(beta2=1.0), "beta2"), (dict(beta2=nan), "beta2"),
-                     (dict(eps=0.0), "eps"), (dict(eps=-1e-8), "eps"), (dict(eps=1e-60), "eps"), (dict(eps=nan), "eps"),
+                     (dict(eps=0.0), "eps"), (dict(eps=-1e-8), "eps"), (dict(eps=1e-60), "eps"), (dict(eps=1e-31), "eps"), (dict(eps=inf), "eps"), (dict(eps=nan), "eps"),
                      (dict(step=0), "steps count"), (dict(step=-3), "steps count"), (dict(plan_ptr=None), "null"),
                      (dict(plan_ptr=4100), "misaligned")):
         refused(step(**kw), text)
