@@ -187,10 +187,7 @@ __device__ __forceinline__ void put(T* p, int i, int n, const Four<T>& r) {
     } else if constexpr (sizeof(T) == 2) {
       *(u32x2_any*)(p + i) = r.w;
     } else {
-      if (STREAM)
-        __builtin_nontemporal_store(r.w, (u32_any*)(p + i));
-      else
-        *(u32_any*)(p + i) = r.w;
+      *(u32_any*)(p + i) = r.w;  // (codes: a quarter of the bytes of what they stand for may stay in the cache)
     }
   } else {
     T e[kEach];
@@ -349,7 +346,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Chunk* __restrict
     step_chunk<_Float16, BITS, STREAM>(c, a, s);
 }
 
-// eight elements a thread: 16 bytes of each output
+// Eight elements a thread: 16 bytes of each output, past the caches (it goes to a checkpoint; a table of 25.3 M, step
+// and read-out: 98 -> 91 us).
 template <bool EDGE, int N>
 __device__ __forceinline__ void read_pieces(const Chunk& c, __bf16* out_m, __bf16* out_v, int first) {
   constexpr int kStep = 2 * kThreads * kEach;
@@ -384,8 +382,8 @@ __device__ __forceinline__ void read_pieces(const Chunk& c, __bf16* out_m, __bf1
       u32x4 wm, wv;
       __builtin_memcpy(&wm, em, sizeof(em));
       __builtin_memcpy(&wv, ev, sizeof(ev));
-      *(u32x4_any*)(out_m + i) = wm;
-      *(u32x4_any*)(out_v + i) = wv;
+      __builtin_nontemporal_store(wm, (u32x4_any*)(out_m + i));
+      __builtin_nontemporal_store(wv, (u32x4_any*)(out_v + i));
     } else {
 #pragma unroll
       for (int j = 0; j < 2 * kEach; ++j)

@@ -20,9 +20,9 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
 
-// How rows are read and written.  kStream: past the caches.  A pass over more than the Infinity Cache holds (256 MB)
-// leaves nothing in it that the next kernel would find (1024 x 65536 fp32 forward 98 -> 91 us, 512 x 65536 backward 80
-// -> 72), a smaller one might (and gains nothing: 1001 x 4099 fp16 9.0 -> 9.35).
+// How rows are read and written.  kStream: past the caches, for a pass over more than half of the Infinity Cache
+// (256 MB), of which its neighbours would find little there: by 3 to 14 % faster from 150 MB on (forward 1024 x 65536 fp32
+// 98 -> 91 us, backward 512 x 65536 80 -> 73, 2496 x 16384 bf16 56 -> 54), even at 100 MB, up to 20 % slower at 60 MB.
 enum { kPlain, kStream };
 
 // The pieces of a row that a thread holds.  Element j of piece k is column c[k] + j and counts where j >= skip[k]:
@@ -668,7 +668,7 @@ Shape shape_of(int cols, int vec, int wave) {
   return {0, 0, kMaxWaves};
 }
 
-bool streams(int64_t rows, int cols, int passes, size_t size) { return (double)rows * cols * passes * size > 256e6; }
+bool streams(int64_t rows, int cols, int passes, size_t size) { return (double)rows * cols * passes * size > 128e6; }
 
 // blocks that are all on the chip at once (`waves` to each, `room` of them to a SIMD) and have as many turns each
 int64_t blocks_of(int64_t turns, int waves, int room) {
