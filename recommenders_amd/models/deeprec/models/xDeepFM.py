@@ -5,7 +5,16 @@
 linear / FM / CIN / DNN parts summed into the logit -- but as an ``XDeepFMEngine`` that runs
 hand-written HIP kernels on MI355X (see ``_engine.py`` and ``include/xdfm.h``).
 
-One additional, optional hyper-parameter is understood:
+Additional, optional hyper-parameters are understood:
+
+``enable_LN`` (bool, default False)
+    A layer norm (with weights of its own) behind every product of the DNN tower, in front of dropout and activation,
+    in training and scoring alike.  Excludes ``enable_BN``; served by every ``compute_dtype``.
+``optimizer: adamw``
+    Decoupled weight decay: ``weight_decay`` (default 0.01) of the dense matrices, ``embed_weight_decay`` (default 0.0,
+    ``dense_exact`` only) of the table and the linear weights; vectors do not decay.  ``adamw_state_bits`` (32, default,
+    or 8): 2 bytes of optimizer state per parameter instead of 8.  Under ``sparse_rows`` / ``sparse_lazy`` the table's
+    rows take Adam's row update.  Needs l1 / l2 coefficients of 0 and no ``is_clip_norm``.
 
 ``embedding_update`` (str, default ``"dense_exact"``)
     ``"dense_exact"``: reference semantics -- the table's gradient is dense (regularisers,

@@ -23,7 +23,8 @@ U = 2.0 ** -24
 ACT = {"identity": 0, "relu": 1, "sigmoid": 2, "tanh": 3, "elu": 4}
 TYPES = {"fp32": (torch.float32, 0), "bf16": (torch.bfloat16, 1), "fp16": (torch.float16, 2)}
 SIZES = [(1, 1), (4, 1), (1, 7), (3, 20), (130, 20), (5, 64), (2, 65), (17, 257), (64, 1000), (33, 1024), (9, 2048), (7, 2496),
-         (5, 4097), (3, 8192), (2, 16387), (2, 40001), (4099, 33), (2500, 512)]
+         (5, 4097), (3, 8192), (2, 16387), (2, 40001), (4099, 33), (2500, 512), (70, 200), (45, 700), (300, 129),
+         (1029, 100), (3000, 8), (2, 16384), (600, 2600), (1100, 1600), (20, 6001), (300, 9000)]
 
 
 def half_step(dtype, value):
@@ -303,6 +304,28 @@ def test_two_runs_agree_in_every_bit_and_other_streams_too():
             again = bwd(x, dy, 1, gamma, beta, stats, "elu", dx2)
         side.synchronize()
         assert torch.equal(y, y2) and torch.equal(dx, dx2) and all(torch.equal(a, b) for a, b in zip(ref, again))
+
+
+def test_two_calls_at_once():
+    """Two streams, each with its own workspace, under way together: the same bits as alone."""
+    sets = [make(20000, c, torch.float32, seed=c) for c in (500, 512)]
+    alone = []
+    for x, dy, gamma, beta, _ in sets:
+        y, dx, stats = torch.empty_like(x), torch.empty_like(x), torch.empty((2, 20000), device="cuda")
+        fwd(x, 0, gamma, beta, "sigmoid", y, stats)
+        alone.append((y, stats, dx) + bwd(x, dy, 0, gamma, beta, stats, "sigmoid", dx))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        got = []
+        for s, (x, dy, gamma, beta, _) in zip(streams, sets):
+            with torch.cuda.stream(s):
+                y, dx, stats = torch.empty_like(x), torch.empty_like(x), torch.empty((2, 20000), device="cuda")
+                fwd(x, 0, gamma, beta, "sigmoid", y, stats)
+                got.append((y, stats, dx) + bwd(x, dy, 0, gamma, beta, stats, "sigmoid", dx))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, got):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
 def test_captured_and_replayed():
