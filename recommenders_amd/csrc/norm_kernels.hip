@@ -49,6 +49,14 @@ struct Pieces {
       skip[k] = at - c[k];
     }
   }
+  // whether every piece of the wave counts as a whole: one branch then saves the forward pass four operations an
+  // element (1024 x 65536 bf16 54.7 -> 51.5 us; in the backward pass it gained and lost 1 %)
+  __device__ __forceinline__ bool whole() const {
+    bool all = true;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) all &= skip[k] == 0;
+    return __all(all);
+  }
 };
 
 template <typename T>
@@ -316,7 +324,7 @@ __global__ __launch_bounds__(G ? kThreads : 64 * kMaxWaves) void layer_norm_fwd_
   const int lane = G ? (int)threadIdx.x & (G - 1) : (int)threadIdx.x;
   const int64_t at_once = G ? kThreads / (G ? G : 1) : 1;
   const Pieces<T, NV> at(lane * V, per_row * V, cols);
-  const bool tiny = G == 8 && cols < V;
+  const bool tiny = G == 8 && cols < V, whole = at.whole();
   const float n = (float)cols;
   float g[NV][V], b[NV][V];
   load_weights<T, NV>(gamma, at, tiny, g);
@@ -330,9 +338,10 @@ __global__ __launch_bounds__(G ? kThreads : 64 * kMaxWaves) void layer_norm_fwd_
   for (int64_t r0 = blockIdx.x * at_once; r0 < rows; r0 += stride, r += stride) {
     float v[NV][V], s[1] = {0.f};
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      unpack<T>(raw[k], v[k]);
-      mask(v[k], at.skip[k]);
+    for (int k = 0; k < NV; ++k) unpack<T>(raw[k], v[k]);
+    if (!whole) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) mask(v[k], at.skip[k]);
     }
     if (r0 + stride < rows)  // the next row is under way while this one is worked on
       load_row<MODE, T, NV>(x + (r + stride < rows ? r + stride : rows - 1) * xs, at, tiny, raw);
@@ -346,10 +355,15 @@ __global__ __launch_bounds__(G ? kThreads : 64 * kMaxWaves) void layer_norm_fwd_
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        v[k][j] -= mean;
-        q[0] += j >= at.skip[k] ? v[k][j] * v[k][j] : 0.f;
-      }
+      for (int j = 0; j < V; ++j) v[k][j] -= mean;
+    if (!whole) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) mask(v[k], at.skip[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) q[0] = fmaf(v[k][j], v[k][j], q[0]);
     row_sum<G>(q, waves, sh[1]);
     const float rstd = 1.f / sqrtf(q[0] / n + eps);
 #pragma unroll
