@@ -439,13 +439,13 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_fwd_long_kernel(
 // ------------------------------------------------------------------ backward
 // x and dy are read once and dx is written: a thread keeps its columns from row to row, so it carries their dgamma and
 // dbeta along in registers.  A block works on blockDim / (lanes of a row) rows at once; at the end it adds up what its
-// row groups hold (pairwise, through LDS) and leaves one partial sum per column in part[0 or 1][block][column].
+// row groups hold (pairwise, through LDS) and leaves one partial sum per column in part_g, part_b [block][column].
 // `waves`: of a row, for G = 0.  Dynamic LDS: blockDim / 2 * NV * V * 2 floats.
 template <typename T, int G, int NV, int MODE>
 __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
     const T* x, int64_t xs, const T* dy, int64_t dys, int64_t rows, int cols, const float* __restrict__ gamma,
     const float* __restrict__ beta, const float* __restrict__ stats, int act, T* dx, int64_t dxs,
-    float* __restrict__ part, int waves) {
+    float* __restrict__ part_g, float* __restrict__ part_b, int waves) {
   constexpr int V = kVec<T>;
   __shared__ float sh[2][kMaxWaves][2];
   extern __shared__ float acc[];
@@ -553,8 +553,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
     groups = half;
   }
   if (holder && number == 0) {
-    float* pg = part + (int64_t)blockIdx.x * cols;
-    float* pb = part + (int64_t)(gridDim.x + blockIdx.x) * cols;
+    float* pg = part_g + (int64_t)blockIdx.x * cols;
+    float* pb = part_b + (int64_t)blockIdx.x * cols;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
       if (at.skip[k] < V) {
@@ -742,25 +742,31 @@ void fwd_as(const void* x, int64_t xs, int64_t rows, int cols, const float* gamm
 // waves a block 1024; 512 columns of bf16 by 16384 rows: 14.6 against 16.6 us; 2496 columns, 5 waves a row: 56 against
 // 108).  Where that would leave CUs without a block, 8 (20 x 8192 fp32: 7.3 against 8.2 us; 65536 rows: 9.0 and 8.9).
 constexpr int kBwdWaves = kMaxWaves;
+// Turns up to which one block takes all rows and writes dgamma and dbeta itself, without a second launch: 128 x 20 fp32
+// 4.8 against 7.1 us, two turns 16 x 1024 7.05 against 7.6, four turns 32 x 1024 10.7 against 7.6.
+constexpr int kTurnsOfOne = 2;
 
-// the number of partial sums that lie in ws afterwards
+// the number of partial sums that lie in ws afterwards (0: dgamma and dbeta are written)
 template <typename T, int MODE>
 int bwd_as(const void* x, int64_t xs, const void* dy, int64_t dys, int64_t rows, int cols, const float* gamma,
-           const float* beta, const float* stats, int act, void* dx, int64_t dxs, float* ws, hipStream_t st) {
+           const float* beta, const float* stats, int act, void* dx, int64_t dxs, float* dgamma, float* dbeta, float* ws,
+           hipStream_t st) {
   // 8 elements a thread: with their weights and the weights' gradients they take 6 registers each
   constexpr int kWave = 8 / kVec<T>;
   const Shape s = shape_of(cols, kVec<T>, kWave);
   const int per_row = s.group ? s.group : 64 * s.waves;
   const int at_most = kBwdWaves * 64 / per_row;
-  const int at_once = s.group && ceil_div(rows, at_most) < kCus ? at_most / 2 : at_most;
+  const bool one = ceil_div(rows, at_most) <= kTurnsOfOne;
+  const int at_once = !one && s.group && ceil_div(rows, at_most) < kCus ? at_most / 2 : at_most;
   const int threads = at_once * per_row;
-  const int64_t blocks = blocks_of(ceil_div(rows, at_once), threads / 64, 4);
+  const int64_t blocks = one ? 1 : blocks_of(ceil_div(rows, at_once), threads / 64, 4);
+  float *part_g = one ? dgamma : ws, *part_b = one ? dbeta : ws + blocks * cols;
 #define CASE(G, NV)                                                                                                \
   if (s.group == G && s.pieces == NV) {                                                                            \
     XDFM_LAUNCH("layer_norm_bwd_kernel", st, (layer_norm_bwd_kernel<T, G, NV, MODE>), dim3((unsigned)blocks),      \
                 dim3((unsigned)threads), (size_t)threads* NV* kVec<T> * sizeof(float), (const T*)x, xs,            \
-                (const T*)dy, dys, rows, cols, gamma, beta, stats, act, (T*)dx, dxs, ws, s.waves);                 \
-    return (int)blocks;                                                                                            \
+                (const T*)dy, dys, rows, cols, gamma, beta, stats, act, (T*)dx, dxs, part_g, part_b, s.waves);     \
+    return one ? 0 : (int)blocks;                                                                                  \
   }
   CASE(8, 1) CASE(16, 1) CASE(32, 1) CASE(64, 1)
   if constexpr (kWave == 2) {
@@ -789,9 +795,10 @@ void fwd(const void* x, int64_t xs, int64_t rows, int cols, const float* gamma, 
 
 template <typename T>
 int bwd(const void* x, int64_t xs, const void* dy, int64_t dys, int64_t rows, int cols, const float* gamma,
-        const float* beta, const float* stats, int act, void* dx, int64_t dxs, float* ws, hipStream_t st) {
+        const float* beta, const float* stats, int act, void* dx, int64_t dxs, float* dgamma, float* dbeta, float* ws,
+        hipStream_t st) {
   return (streams(rows, cols, 3, sizeof(T)) ? bwd_as<T, kStream> : bwd_as<T, kPlain>)(
-      x, xs, dy, dys, rows, cols, gamma, beta, stats, act, dx, dxs, ws, st);
+      x, xs, dy, dys, rows, cols, gamma, beta, stats, act, dx, dxs, dgamma, dbeta, ws, st);
 }
 
 }  // namespace
@@ -843,18 +850,22 @@ extern "C" int xdfm_layer_norm_bwd(const void* x, int64_t x_stride, const void* 
   XDFM_REQUIRE((dx != dy || dx_stride == dy_stride) && (dx != x || dx_stride == x_stride),
                "xdfm_layer_norm_bwd: dx on dy or x needs the same stride");
   hipStream_t st = (hipStream_t)stream;
-  int parts = 0;  // no rows: sums of nothing
+  int parts = 0;
   if (rows == 0)
-    ;
+    ;  // sums of nothing
   else if (dtype == XDFM_F32)
-    parts = bwd<float>(x, x_stride, dy, dy_stride, rows, cols, gamma, beta, stats, act, dx, dx_stride, workspace, st);
+    parts = bwd<float>(x, x_stride, dy, dy_stride, rows, cols, gamma, beta, stats, act, dx, dx_stride, dgamma, dbeta,
+                       workspace, st);
   else if (dtype == XDFM_BF16)
-    parts = bwd<__bf16>(x, x_stride, dy, dy_stride, rows, cols, gamma, beta, stats, act, dx, dx_stride, workspace, st);
+    parts = bwd<__bf16>(x, x_stride, dy, dy_stride, rows, cols, gamma, beta, stats, act, dx, dx_stride, dgamma, dbeta,
+                        workspace, st);
   else
-    parts = bwd<_Float16>(x, x_stride, dy, dy_stride, rows, cols, gamma, beta, stats, act, dx, dx_stride, workspace, st);
-  XDFM_LAUNCH("layer_norm_bwd_finish_kernel", st, layer_norm_bwd_finish_kernel,
-              dim3((unsigned)ceil_div(cols, kFinish), 2), dim3(kFinish, kFinish), 0, workspace, parts, cols, dgamma,
-              dbeta);
+    parts = bwd<_Float16>(x, x_stride, dy, dy_stride, rows, cols, gamma, beta, stats, act, dx, dx_stride, dgamma, dbeta,
+                          workspace, st);
+  if (parts || rows == 0)
+    XDFM_LAUNCH("layer_norm_bwd_finish_kernel", st, layer_norm_bwd_finish_kernel,
+                dim3((unsigned)ceil_div(cols, kFinish), 2), dim3(kFinish, kFinish), 0, workspace, parts, cols, dgamma,
+                dbeta);
   XDFM_LAUNCH_CHECK();
   return XDFM_OK;
 }
