@@ -672,7 +672,7 @@ __global__ __launch_bounds__(kFinish* kFinish) void layer_norm_bwd_finish_kernel
 
 // ------------------------------------------------------------------ which kernel, how many blocks
 constexpr int kCus = 256;
-constexpr int kMaxParts = 4 * kCus;
+constexpr int kMaxParts = 2 * kCus;  // backward blocks of 8 waves or more at 4 waves a SIMD: 2 at most on a CU
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

@@ -803,6 +803,7 @@ class XDeepFMEngine(object):
             _lib.check(self.lib.xdfm_dense_bwd_workspace_floats(B, final_len, 1, ctypes.byref(sz)))
             part_floats = max(part_floats, sz.value)
         dnn_part_floats = 1
+        ln_floats = 1
         if hp.use_DNN_part:
             last = F * D
             for k, size in enumerate(hp.layer_sizes):
@@ -815,7 +816,7 @@ class XDeepFMEngine(object):
                 if self.use_ln:
                     buf("ln_stats_%d" % k, 2 * B)
                     _lib.check(self.lib.xdfm_layer_norm_bwd_workspace_floats(B, int(size), ctypes.byref(sz)))
-                    dnn_part_floats = max(dnn_part_floats, sz.value)
+                    ln_floats = max(ln_floats, sz.value)
                 if self.use_dropout:
                     buf("drop_%d" % k, B, int(size))
                 _lib.check(self.lib.xdfm_dense_bwd_workspace_floats(B, last, int(size), ctypes.byref(sz)))
@@ -828,6 +829,7 @@ class XDeepFMEngine(object):
             _lib.check(self.lib.xdfm_dense_bwd_workspace_floats(B, last, 1, ctypes.byref(sz)))
             dnn_part_floats = max(dnn_part_floats, sz.value)
         buf("part", max(part_floats, 1))
+        buf("ln_part", ln_floats)
         if self.bf16:
             buf("bf16_ws", bf16_floats)
         # the DNN tower runs on its own stream beside the CIN: its partial sums get their own space
@@ -1265,7 +1267,7 @@ class XDeepFMEngine(object):
             self.lib.xdfm_layer_norm_bwd(_ptr(x), n, _ptr(dy), n, 0, B, n, _ptr(self.views["ln_dnn_g_%d" % k]),
                                          _ptr(self.views["ln_dnn_o_%d" % k]), _ptr(self.ws["ln_stats_%d" % k]), act,
                                          _ptr(dy), n, _ptr(self.grad_views["ln_dnn_g_%d" % k]),
-                                         _ptr(self.grad_views["ln_dnn_o_%d" % k]), _ptr(self.ws["part_dnn"]),
+                                         _ptr(self.grad_views["ln_dnn_o_%d" % k]), _ptr(self.ws["ln_part"]),
                                          self._stream())
         )
 
@@ -1426,10 +1428,10 @@ class XDeepFMEngine(object):
         return jobs
 
     def _dnn_plain(self):
-        """No dropout, norm or softmax in the tower: its backward splits into an input-gradient
+        """No dropout, batch norm or softmax in the tower: its backward splits into an input-gradient
         chain and the weight gradients."""
         hp = self.hp
-        return not (self._dropout_live or self.use_bn or self.use_ln
+        return not (self._dropout_live or self.use_bn
                     or any(_ACT[hp.activation[k]] == _SOFTMAX for k in range(len(hp.layer_sizes))))
 
     def _dnn_backward(self, B, first_layer_dx, phase="all", head_jobs=False):
@@ -1460,12 +1462,16 @@ class XDeepFMEngine(object):
         if phase != "all":
             x_in, K_in = acts[-1], sizes[-1]
             layers = [(x_in, self.views["dnn_w_out"], ws["dnn_out"], g, K_in, 1, 0, d_acts[-1], 0,
-                       gv["dnn_w_out"], gv["dnn_b_out"])]
+                       gv["dnn_w_out"], gv["dnn_b_out"], None)]
             for k in range(n_layers - 1, -1, -1):
                 dx, acc = (first_layer_dx if first_layer_dx is not None else (None, 0)) if k == 0 else (d_acts[k], 0)
                 layers.append((acts[k], self.views["dnn_w_%d" % k], acts[k + 1], d_acts[k + 1], sizes[k], sizes[k + 1],
-                               _ACT[hp.activation[k]], dx, acc, gv["dnn_w_%d" % k], gv["dnn_b_%d" % k]))
-            for (x, w, y, dy, K, Nout, act, dx, acc, dw, db) in layers:
+                               _ACT[hp.activation[k]], dx, acc, gv["dnn_w_%d" % k], gv["dnn_b_%d" % k], k))
+            for (x, w, y, dy, K, Nout, act, dx, acc, dw, db, k) in layers:
+                if self.use_ln and k is not None:  # (part of the chain of input gradients: dy in place)
+                    if want_dx:
+                        self._ln_bwd(ws["z_%d" % k], dy, k, B, Nout, act)
+                    act = 0
                 if want_dx and dx is None:
                     continue
                 _lib.check(
