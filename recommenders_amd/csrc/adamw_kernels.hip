@@ -65,7 +65,7 @@ struct Step {
 
 __device__ __forceinline__ Step step_of(const Args& a) {
   if (!a.state) return {a.step, a.inv_root, a.t};
-  const float t = a.state[3];
+  const float t = fmaxf(a.state[3], 1.f);  // (a state that was not advanced yet: the first step)
   return {a.lr / -expm1f(t * a.log_b1), 1.f / sqrtf(-expm1f(t * a.log_b2)), (uint32_t)t};
 }
 

@@ -349,6 +349,39 @@ def test_step_count_from_the_device_equals_the_hosts():
             b.check_step(before, 0.01, t, seed=9)
 
 
+def test_a_step_count_that_was_not_advanced_counts_as_the_first():
+    a, b = Setup([500, 70], 8, seed=2), Setup([500, 70], 8, seed=2)
+    a.opt.step(lr=0.01, opt_state=torch.tensor([1.0, 1.0, 0.0, 0.0], device="cuda"), seed=9)
+    b.opt.step(lr=0.01, opt_state=torch.tensor([0.9, 0.999, 0.0, 1.0], device="cuda"), seed=9)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(a.p + a.m + a.v, b.p + b.m + b.v))
+    for bad in (torch.zeros(3, device="cuda"), torch.zeros(4), torch.zeros(4, device="cuda", dtype=torch.float64),
+                torch.zeros(8, device="cuda")[::2]):
+        with pytest.raises(ValueError, match="opt_state"):
+            a.opt.step(lr=0.01, opt_state=bad)
+    with pytest.raises(ValueError, match="either"):
+        a.opt.step(lr=0.01)
+    with pytest.raises(ValueError, match="elements of"):
+        a.opt.read_state(torch.zeros(5, device="cuda", dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_class_refuses_tensors_that_do_not_fit(bits):
+    n = 100
+    p, g = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    for kw in (dict(params=[p.double()]), dict(grads=[g.double()]), dict(grads=[g[:50]]), dict(params=[p.repeat(2)[::2]]),
+               dict(grads=[g.cpu()]), dict(slot_m=[p.half()]), dict(slot_v=[]), dict(weight_decay=[0.1, 0.1])):
+        a = dict(params=[p], grads=[g], state_bits=bits)
+        a.update(kw)
+        with pytest.raises(ValueError):
+            AdamW(**a)
+    # the library's own refusals come through
+    with pytest.raises(_lib.XdfmError, match="overlap"):
+        AdamW([p, p], [g, g], state_bits=bits)
+    with pytest.raises(_lib.XdfmError, match="gradient"):
+        AdamW([p], [p], state_bits=bits)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_captured_and_replayed_with_two_optimizers(bits):
     """Two graphs of two optimizers, replayed in turn with eager steps of twins and waits between: equal in every bit."""
