@@ -482,9 +482,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
     float xh[NV][V], t[NV][V], s[2] = {0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      xw[k] = xn[k];
+      // (a group past the last row adds nothing to any sum: dy = 0, and x = 0 because dx may lie on x, so that what
+      // it read there can be the last row's dx already, and infinite)
+      const u32x4 none = {0u, 0u, 0u, 0u};
+      xw[k] = live ? xn[k] : none;
       unpack<T>(dn[k], t[k]);
-      mask(t[k], live ? at.skip[k] : V);  // with dy = 0 they add nothing to any sum
+      mask(t[k], live ? at.skip[k] : V);
     }
     if (r0 + stride < rows) fetch(r + stride);  // the next row is under way while this one is worked on
 #pragma unroll

@@ -226,6 +226,24 @@ def test_in_place_equals_out_of_place(cols, kind):
         assert torch.equal(dy2 if target == "dy" else x2, dx) and torch.equal(dg, dg2) and torch.equal(db, db2)
 
 
+@pytest.mark.parametrize("rows,cols", [(257, 20), (4099, 100), (2049, 512), (1003, 2496)])
+def test_infinite_dx_on_x_stays_out_of_the_weights_gradients(rows, cols):
+    """dx beyond the type's range, written where x was: other rows' threads that look past the last row see it there."""
+    x, dy, gamma, beta, view = make(rows, cols, torch.float16, 31)
+    dy *= 3e4
+    gamma = gamma.abs() * 100  # dx ~ 3e3 * 100 * rstd
+    mean, rstd = stats_exact(x)
+    stats = torch.cat([mean, rstd], 1).t().float().contiguous()
+    out = torch.empty_like(x)
+    dg, db = bwd(x, dy, 2, gamma, beta, stats, "identity", out)
+    assert torch.isinf(out).any() and torch.isfinite(dg).all() and torch.isfinite(db).all()
+    for _ in range(3):
+        on = x.clone()
+        dg2, db2 = bwd(on, dy, 2, gamma, beta, stats, "identity", on)
+        torch.cuda.synchronize()
+        assert torch.equal(on, out) and torch.equal(dg2, dg) and torch.equal(db2, db)
+
+
 def test_no_rows_and_rows_without_spread():
     gamma, beta = torch.randn(50, device="cuda"), torch.randn(50, device="cuda")
     x = torch.empty((0, 50), device="cuda")
