@@ -10,7 +10,7 @@
 // once and walk the rows, so that gamma, beta and the weights' gradients stay with a thread's columns.
 //   1024 x 65536 fp32 relu, forward     91 us, 5.9 TB/s of 6.2 that a plain streaming addition reaches
 //    512 x 65536 fp32 relu, backward    73 us, 5.5 TB/s, 5 of them in the second launch that joins 256 partial sums
-//   2496 x 16384 bf16, backward         54 us, 4.5 TB/s: 5 waves a row wait for each other at its two sums
+//   2496 x 16384 bf16, backward         47.5 us, 5.2 TB/s, 5 of them in the second launch
 // Rows longer than the registers of 16 waves (16384 elements forward, 8192 backward) take a slower way (2.2 to 2.9 TB/s).
 #include <hip/hip_runtime.h>
 
@@ -31,7 +31,7 @@ constexpr int kVec = 16 / (int)sizeof(T);
 
 // How rows are read and written.  kStream: past the caches, for a pass over more than half of the Infinity Cache
 // (256 MB), of which its neighbours would find little there: by 3 to 14 % faster from 150 MB on (forward 1024 x 65536 fp32
-// 98 -> 91 us, backward 512 x 65536 80 -> 73, 2496 x 16384 bf16 56 -> 54), even at 100 MB, up to 20 % slower at 60 MB.
+// 98 -> 91 us, backward 512 x 65536 80 -> 73), even at 100 MB, up to 20 % slower at 60 MB.
 enum { kPlain, kStream };
 
 // The pieces of a row that a thread holds.  Element j of piece k is column c[k] + j and counts where j >= skip[k]:
@@ -72,6 +72,11 @@ template <int V>
 __device__ __forceinline__ void mask(float (&v)[V], int skip) {
 #pragma unroll
   for (int j = 0; j < V; ++j) v[j] = j >= skip ? v[j] : 0.f;
+}
+
+template <int MODE>
+__device__ __forceinline__ u32x4 load_16(const void* from) {
+  return MODE == kStream ? __builtin_nontemporal_load((const u32x4_any*)from) : *(const u32x4_any*)from;
 }
 
 template <int MODE, typename T, int NV>
@@ -567,6 +572,145 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
   }
 }
 
+// Rows of 16 bits and 2 to 5 pieces a lane, each in one wave: its sums need no barrier, and eight waves of up to 256
+// registers have more bytes under way (80 KB of a CU's reads at 5 pieces) than the sixteen that hold 8 elements a thread
+// (30 KB).  What is not needed all the time makes room for that: gamma and beta lie in LDS, xhat is formed again for dx.
+// 2496 x 16384 bf16 47.5 against 53.5 us, with tanh 59 and 74; 640 columns 16.7 and 21.3; 1024 rows of 2496 11.1 and 12.3,
+// 256 rows, where few CUs have a block, 9.5 and 8.9.  (fp32, whose rows are under way in twice the bytes as it is: 1024
+// columns 40 against 37 us.)
+constexpr int kRowWaves = 8, kMostAlone = 5;
+template <typename T, int NV, int MODE, bool ACT>
+__global__ __launch_bounds__(64 * kRowWaves) void layer_norm_bwd_wave_kernel(
+    const T* x, int64_t xs, const T* dy, int64_t dys, int64_t rows, int cols, const float* __restrict__ gamma,
+    const float* __restrict__ beta, const float* __restrict__ stats, int act, T* dx, int64_t dxs,
+    float* __restrict__ part_g, float* __restrict__ part_b) {
+  constexpr int V = kVec<T>;
+  __shared__ u32x4 weights[2][NV][V / 4][64];
+  __shared__ float acc[2][kRowWaves][2 * V][64 + 64 / V];  // (read V apart: the padding spreads them over the banks)
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+  const Pieces<T, NV> at(lane * V, 64 * V, cols);
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if (wave == k) {
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i) {
+        weights[0][k][i][lane] = *reinterpret_cast<const u32x4_any*>(gamma + at.c[k] + 4 * i);
+        weights[1][k][i][lane] = *reinterpret_cast<const u32x4_any*>(beta + at.c[k] + 4 * i);
+      }
+    }
+  __syncthreads();
+  const auto weight = [&](int which, int k, int l, float (&v)[1][V]) {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      const u32x4 w = weights[which][k][i][l];
+      __builtin_memcpy(&v[0][4 * i], &w, 16);
+    }
+  };
+  uint32_t byte[NV];  // of the pieces in their row (32 bits, so that the row's address stays in scalar registers)
+#pragma unroll
+  for (int k = 0; k < NV; ++k) byte[k] = (uint32_t)at.c[k] * (uint32_t)sizeof(T);
+  const float n = (float)cols;
+  float sg[NV][V], sb[NV][V];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) sg[k][j] = sb[k][j] = 0.f;
+  const int64_t stride = (int64_t)gridDim.x * kRowWaves;
+  int64_t r = (int64_t)blockIdx.x * kRowWaves + wave;
+  u32x4 xn[NV], dn[NV];
+  float mean_n = 0.f, rstd_n = 0.f;
+  const auto fetch = [&](int64_t row) {
+    const char *xr = (const char*)(x + row * xs), *dr = (const char*)(dy + row * dys);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) xn[k] = load_16<MODE>(xr + byte[k]);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) dn[k] = load_16<MODE>(dr + byte[k]);
+    mean_n = stats[row];
+    rstd_n = stats[rows + row];
+  };
+  if (r < rows) fetch(r);
+  for (; r < rows; r += stride) {
+    const float mean = mean_n, rstd = rstd_n;
+    u32x4 xw[NV], dw[NV];
+    float t[NV][V], s[2] = {0.f, 0.f};
+    int l = lane;
+    asm volatile("" : "+v"(l));  // (this and the others below: or the compiler keeps the weights and xhat in registers
+                                 // all the same, and leaves the sums to the loop's end with all that goes into them)
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      xw[k] = xn[k];
+      dw[k] = dn[k];
+    }
+    if (r + stride < rows) fetch(r + stride);  // the next row is under way while this one is worked on
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      __builtin_amdgcn_sched_barrier(0);
+      float xh[1][V], g[1][V], d[1][V];
+      unpack<T>(xw[k], xh[0]);
+      weight(0, k, l, g);
+#pragma unroll
+      for (int j = 0; j < V; ++j) xh[0][j] = (xh[0][j] - mean) * rstd;
+      asm volatile("" : "+v"(dw[k]));
+      unpack<T>(dw[k], d[0]);
+      if (k == NV - 1) mask(d[0], at.skip[k]);
+      if constexpr (ACT) {
+        float b[1][V];
+        const u32x4 xk[1] = {xw[k]};
+        weight(1, k, l, b);
+        through_act<T>(d, xh, xk, g, b, mean, rstd, act);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        sg[k][j] = fmaf(d[0][j], xh[0][j], sg[k][j]);
+        sb[k][j] += d[0][j];
+        asm volatile("" : "+v"(sg[k][j]), "+v"(sb[k][j]));
+        t[k][j] = d[0][j] * g[0][j];
+        s[0] += t[k][j];
+        s[1] = fmaf(t[k][j], xh[0][j], s[1]);
+      }
+      asm volatile("" : "+v"(s[0]), "+v"(s[1]));
+    }
+    row_sum<64, 2>(s, 1, nullptr);
+    const float a = -(s[0] / n) * rstd, b = -(s[1] / n) * rstd * rstd;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      float x0[V];
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" : "+v"(xw[k]));
+      unpack<T>(xw[k], x0);
+#pragma unroll
+      for (int j = 0; j < V; ++j) t[k][j] = fmaf(t[k][j], rstd, fmaf(x0[j] - mean, b, a));
+      T* to = (T*)((char*)(dx + r * dxs) + byte[k]);
+      if (k < NV - 1)
+        store_piece<MODE, T, V>(to, 0, t[k]);
+      else if (at.skip[k] < V)
+        store_piece<MODE, T, V>(to, at.skip[k], t[k]);
+    }
+  }
+  // the waves' sums, a piece at a time through one of two buffers: [wave][sum][lane] -> one sum per column
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      acc[k & 1][wave][j][lane] = sg[k][j];
+      acc[k & 1][wave][V + j][lane] = sb[k][j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2 * V * 64; i += 64 * kRowWaves) {
+      const int e = i + (int)threadIdx.x;
+      if (e >= 2 * V * 64) break;
+      // neighbours in a block take neighbouring columns of one of the two sums
+      const int which = e / (V * 64), rest = e % (V * 64), l = rest / V, j = rest % V;
+      const int at0 = l * V + k * 64 * V, c = min(at0, cols - V), skip = at0 - c;
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kRowWaves; ++w) sum += acc[k & 1][w][which * V + j][l];
+      if (j >= skip) (which ? part_b : part_g)[(int64_t)blockIdx.x * cols + c + j] = sum;
+    }
+  }
+}
+
 // A piece of a long row: du in t, xhat in xh, and what counts of it.
 template <typename T>
 struct LongPiece {
@@ -684,15 +828,15 @@ struct Shape {
   int group, pieces, waves;
 };
 
-// A row is held by as few lanes as one 16-byte piece each covers; from 64 lanes on by one wave with up to `wave`
+// A row is held by as few lanes as one 16-byte piece each covers; from 64 lanes on by one wave with up to `alone`
 // pieces a lane (its sums need no barrier); then by several waves with `wave` pieces a thread.  pieces = 0: too long
 // for the registers of 16 waves.
-Shape shape_of(int cols, int vec, int wave) {
+Shape shape_of(int cols, int vec, int alone, int wave) {
   const int64_t need = ceil_div(cols, vec);
   if (need <= 8) return {8, 1, 1};
   if (need <= 16) return {16, 1, 1};
   if (need <= 32) return {32, 1, 1};
-  if (need <= 64 * wave) return {64, (int)ceil_div(need, 64), 1};
+  if (need <= 64 * alone) return {64, (int)ceil_div(need, 64), 1};
   if (need <= 64 * kMaxWaves * wave) return {0, wave, (int)ceil_div(need, 64 * wave)};
   return {0, 0, kMaxWaves};
 }
@@ -718,12 +862,17 @@ bool extent_ok(int64_t rows, int64_t stride, int cols) {
 template <typename T, int MODE>
 void fwd_as(const void* x, int64_t xs, int64_t rows, int cols, const float* gamma, const float* beta, float eps, int act,
          void* y, int64_t ys, float* stats, hipStream_t st) {
-  // 16 elements a thread
-  constexpr int kWave = 16 / kVec<T>;
-  const Shape s = shape_of(cols, kVec<T>, kWave);
+  // 16 elements a thread; up to 24 where they hold the row without company (16384 x 1536 bf16 17.5 against 19.2 us, 1100
+  // columns 17.3 and 20.0; with 32 elements, 2048 columns, 29.2 and 24.7).  40 of 16 bits do better than three waves that
+  // a row fills by four fifths, if there are enough of them (2496 x 16384 bf16 30.8 and 32.2 us, with tanh 42 and 53;
+  // 1024 rows 5.4 and 4.9).
+  constexpr int kWave = 16 / kVec<T>, kMore = 40 / kVec<T>;
+  Shape s = shape_of(cols, kVec<T>, 24 / kVec<T>, kWave);
+  if (sizeof(T) == 2 && rows >= 4096 && ceil_div(cols, 64 * kVec<T>) == kMore) s = {64, kMore, 1};
   const dim3 block(s.group ? kThreads : 64 * s.waves);
   const int64_t turns = s.group ? ceil_div(rows, kThreads / s.group) : rows;
-  const dim3 grid((unsigned)blocks_of(turns, (int)block.x / 64, s.pieces * kVec<T> > 8 ? 4 : s.pieces ? 7 : 8));
+  const int each = s.pieces * kVec<T>, room = each > 24 ? 2 : each > 16 ? 3 : each > 8 ? 4 : each ? 7 : 8;
+  const dim3 grid((unsigned)blocks_of(turns, (int)block.x / 64, room));
 #define CASE(G, NV)                                                                                              \
   if (s.group == G && s.pieces == NV) {                                                                          \
     XDFM_LAUNCH("layer_norm_fwd_kernel", st, (layer_norm_fwd_kernel<T, G, NV, MODE>), grid, block, 0, (const T*)x, \
@@ -732,9 +881,9 @@ void fwd_as(const void* x, int64_t xs, int64_t rows, int cols, const float* gamm
   }
   CASE(8, 1) CASE(16, 1) CASE(32, 1) CASE(64, 1) CASE(64, 2)
   if constexpr (kWave == 4) {
-    CASE(64, 3) CASE(64, 4) CASE(0, 4)
+    CASE(64, 3) CASE(64, 4) CASE(64, 5) CASE(64, 6) CASE(0, 4)
   } else {
-    CASE(0, 2)
+    CASE(64, 3) CASE(64, kMore) CASE(0, 2)
   }
 #undef CASE
   XDFM_LAUNCH("layer_norm_fwd_long_kernel", st, layer_norm_fwd_long_kernel<T>, grid, block, 0, (const T*)x, xs, rows,
@@ -754,9 +903,26 @@ template <typename T, int MODE>
 int bwd_as(const void* x, int64_t xs, const void* dy, int64_t dys, int64_t rows, int cols, const float* gamma,
            const float* beta, const float* stats, int act, void* dx, int64_t dxs, float* dgamma, float* dbeta, float* ws,
            hipStream_t st) {
+  const int alone = (int)ceil_div(cols, 64 * kVec<T>);
+  if (sizeof(T) == 2 && alone >= 2 && alone <= kMostAlone && ceil_div(rows, kRowWaves) >= kCus / 2) {
+    const int64_t blocks = blocks_of(ceil_div(rows, kRowWaves), kRowWaves, alone == 2 && act == XDFM_ACT_IDENTITY ? 4 : 2);
+    const auto go = [&](auto kernel) {
+      XDFM_LAUNCH("layer_norm_bwd_wave_kernel", st, kernel, dim3((unsigned)blocks), dim3(64 * kRowWaves), 0, (const T*)x,
+                  xs, (const T*)dy, dys, rows, cols, gamma, beta, stats, act, (T*)dx, dxs, ws, ws + blocks * cols);
+    };
+#define CASE(NV)                                                           \
+  if (alone == NV)                                                         \
+    go(act == XDFM_ACT_IDENTITY ? layer_norm_bwd_wave_kernel<T, NV, MODE, false> \
+                                : layer_norm_bwd_wave_kernel<T, NV, MODE, true>);
+    if constexpr (sizeof(T) == 2) {
+      CASE(2) CASE(3) CASE(4) CASE(5)
+    }
+#undef CASE
+    return (int)blocks;
+  }
   // 8 elements a thread: with their weights and the weights' gradients they take 6 registers each
   constexpr int kWave = 8 / kVec<T>;
-  const Shape s = shape_of(cols, kVec<T>, kWave);
+  const Shape s = shape_of(cols, kVec<T>, kWave, kWave);
   const int per_row = s.group ? s.group : 64 * s.waves;
   const int at_most = kBwdWaves * 64 / per_row;
   const bool one = ceil_div(rows, at_most) <= kTurnsOfOne;

@@ -184,6 +184,37 @@ def test_forward_and_backward_match_the_formula(rows, cols, kind):
 
 
 @pytest.mark.parametrize("act", list(ACT))
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows,cols,pad,offset", [(1017, 513, 0, 0), (1031, 1000, 3, 1), (4099, 1024, 0, 0),
+                                                  (1100, 1025, 5, 0), (1024, 1536, 8, 0), (2051, 1537, 0, 3),
+                                                  (1500, 2041, 7, 1), (1019, 2048, 0, 0), (4101, 2049, 0, 1),
+                                                  (4096, 2496, 6, 0), (4200, 2560, 0, 0)])
+def test_many_rows_of_one_wave_each(act, kind, rows, cols, pad, offset):
+    """16 bits, 2 to 5 pieces a lane: out of place, and in place with the same bits."""
+    dtype, code = TYPES[kind]
+    x, dy, gamma, beta, view = make(rows, cols, dtype, seed=rows + cols, pad=pad, offset=offset)
+    y, dx = view(torch.zeros_like(x)), view(torch.zeros_like(x))
+    stats = torch.empty((2, rows), device="cuda")
+    fwd(x, code, gamma, beta, act, y, stats)
+    check_fwd(x, gamma, beta, act, y, stats)
+    dg, db = bwd(x, dy, code, gamma, beta, stats, act, dx)
+    check_bwd(x, dy, gamma, beta, stats, act, dx, dg, db)
+    for target in ("dy", "x"):
+        x2, dy2 = view(x), view(dy)
+        on = dy2 if target == "dy" else x2
+        dg2, db2 = bwd(x2, dy2, code, gamma, beta, stats, act, on)
+        assert torch.equal(on, dx) and torch.equal(dg, dg2) and torch.equal(db, db2)
+    over = view(x)
+    fwd(over, code, gamma, beta, act, over, None)
+    assert torch.equal(over, y)
+    for t in (y, dx, over, on):
+        whole = t._base.reshape(-1) if t._base is not None else t.reshape(-1)
+        gaps = torch.ones_like(whole, dtype=torch.bool)
+        gaps[offset:].view(rows, cols + pad)[:, :cols] = False
+        assert (whole[gaps] == 77).all()
+
+
+@pytest.mark.parametrize("act", list(ACT))
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("cols,pad,offset", [(20, 3, 1), (1001, 6, 3), (512, 0, 1), (2496, 5, 0)])
 def test_strides_and_odd_addresses_leave_the_gaps_alone(act, kind, cols, pad, offset):
