@@ -572,13 +572,14 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
   }
 }
 
-// Rows of 16 bits and 2 to 5 pieces a lane, each in one wave: its sums need no barrier, and eight waves of up to 256
+// Rows of 2 to 5 pieces a lane, each in one wave, foremost of 16 bits: its sums need no barrier, and eight waves of up to 256
 // registers have more bytes under way (80 KB of a CU's reads at 5 pieces) than the sixteen that hold 8 elements a thread
 // (30 KB).  What is not needed all the time makes room for that: gamma and beta lie in LDS, xhat is formed again for dx.
 // 2496 x 16384 bf16 47.5 against 53.5 us, with tanh 59 and 74; 640 columns 16.7 and 21.3; 1024 rows of 2496 11.1 and 12.3,
-// 256 rows, where few CUs have a block, 9.5 and 8.9.  (fp32, whose rows are under way in twice the bytes as it is: 1024
-// columns 40 against 37 us.)
-constexpr int kRowWaves = 8, kMostAlone = 5;
+// 256 rows, where few CUs have a block, 9.5 and 8.9.  fp32, of which those have twice the bytes under way, gains less
+// (640 x 16384 23.2 and 25.3, 1280 x 4096 15.4 and 18.1) and loses where the pass does not stay in the caches (1280 x 65536
+// 182 and 170): 3 to 6 pieces there, and small passes only.
+constexpr int kRowWaves = 8;
 template <typename T, int NV, int MODE, bool ACT>
 __global__ __launch_bounds__(64 * kRowWaves) void layer_norm_bwd_wave_kernel(
     const T* x, int64_t xs, const T* dy, int64_t dys, int64_t rows, int cols, const float* __restrict__ gamma,
@@ -904,8 +905,9 @@ int bwd_as(const void* x, int64_t xs, const void* dy, int64_t dys, int64_t rows,
            const float* beta, const float* stats, int act, void* dx, int64_t dxs, float* dgamma, float* dbeta, float* ws,
            hipStream_t st) {
   const int alone = (int)ceil_div(cols, 64 * kVec<T>);
-  if (sizeof(T) == 2 && alone >= 2 && alone <= kMostAlone && ceil_div(rows, kRowWaves) >= kCus / 2) {
-    const int64_t blocks = blocks_of(ceil_div(rows, kRowWaves), kRowWaves, alone == 2 && act == XDFM_ACT_IDENTITY ? 4 : 2);
+  constexpr bool kAlone = sizeof(T) == 2 || MODE == kPlain;
+  if (kAlone && alone >= (sizeof(T) == 2 ? 2 : 3) && alone <= (sizeof(T) == 2 ? 5 : 6) && ceil_div(rows, kRowWaves) >= kCus / 2) {
+    const int64_t blocks = blocks_of(ceil_div(rows, kRowWaves), kRowWaves, alone * kVec<T> <= (act == XDFM_ACT_IDENTITY ? 16 : 12) ? 4 : 2);
     const auto go = [&](auto kernel) {
       XDFM_LAUNCH("layer_norm_bwd_wave_kernel", st, kernel, dim3((unsigned)blocks), dim3(64 * kRowWaves), 0, (const T*)x,
                   xs, (const T*)dy, dys, rows, cols, gamma, beta, stats, act, (T*)dx, dxs, ws, ws + blocks * cols);
@@ -914,8 +916,13 @@ int bwd_as(const void* x, int64_t xs, const void* dy, int64_t dys, int64_t rows,
   if (alone == NV)                                                         \
     go(act == XDFM_ACT_IDENTITY ? layer_norm_bwd_wave_kernel<T, NV, MODE, false> \
                                 : layer_norm_bwd_wave_kernel<T, NV, MODE, true>);
-    if constexpr (sizeof(T) == 2) {
-      CASE(2) CASE(3) CASE(4) CASE(5)
+    if constexpr (kAlone) {
+      CASE(3) CASE(4) CASE(5)
+      if constexpr (sizeof(T) == 2) {
+        CASE(2)
+      } else {
+        CASE(6)
+      }
     }
 #undef CASE
     return (int)blocks;
