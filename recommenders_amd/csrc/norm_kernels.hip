@@ -319,8 +319,11 @@ __device__ __forceinline__ void through_act(float (&d)[NV][V], const float (&xh)
 // row to row, and with them gamma and beta.  (Re-reading the row for each of the three sums instead, one block a row:
 // 226 against 91 us at 1024 x 65536 fp32.  gamma and beta by single elements instead of 16 bytes: 21 against 6 us at
 // 1001 x 4099 fp16, where most waves see one row.)
+// (Two pieces of 16 bits take 97 registers where five waves a SIMD leave 96 to each: asked for, 1001 x 4099 fp16 tanh 7.35
+// against 7.75 us, 1001 x 5000 7.8 and 9.3.)
 template <typename T, int G, int NV, int MODE>
-__global__ __launch_bounds__(G ? kThreads : 64 * kMaxWaves) void layer_norm_fwd_kernel(
+__global__ __launch_bounds__(G ? kThreads : 64 * kMaxWaves,
+                             G == 64 && NV == 2 && sizeof(T) == 2 ? 5 : 1) void layer_norm_fwd_kernel(
     const T* x, int64_t xs, int64_t rows, int cols, const float* __restrict__ gamma, const float* __restrict__ beta,
     float eps, int act, T* y, int64_t ys, float* __restrict__ stats) {
   constexpr int V = kVec<T>;
@@ -872,7 +875,7 @@ void fwd_as(const void* x, int64_t xs, int64_t rows, int cols, const float* gamm
   if (sizeof(T) == 2 && rows >= 4096 && ceil_div(cols, 64 * kVec<T>) == kMore) s = {64, kMore, 1};
   const dim3 block(s.group ? kThreads : 64 * s.waves);
   const int64_t turns = s.group ? ceil_div(rows, kThreads / s.group) : rows;
-  const int each = s.pieces * kVec<T>, room = each > 24 ? 2 : each > 16 ? 3 : each > 8 ? 4 : each ? 7 : 8;
+  const int each = s.pieces * kVec<T>, room = each > 24 ? 2 : each > 16 ? 3 : each > 8 ? (sizeof(T) == 2 && s.group ? 5 : 4) : each ? 7 : 8;
   const dim3 grid((unsigned)blocks_of(turns, (int)block.x / 64, room));
 #define CASE(G, NV)                                                                                              \
   if (s.group == G && s.pieces == NV) {                                                                          \
