@@ -847,11 +847,13 @@ Shape shape_of(int cols, int vec, int alone, int wave) {
 
 bool streams(int64_t rows, int cols, int passes, size_t size) { return (double)rows * cols * passes * size > 128e6; }
 
-// blocks that are all on the chip at once (`waves` to each, `room` of them to a SIMD) and have as many turns each: with
-// 1024 blocks on 768 places the last 256 took a second round (2496 x 16384 bf16 backward, 118 against 108 us)
+// blocks that are all on the chip at once (`waves` to each, `room` of them to a SIMD): with 1024 blocks on 768 places the
+// last 256 took a second round (2496 x 16384 bf16 backward, 118 against 108 us).  All of those, though only some have a
+// last turn: fewer blocks of equal turns leave CUs a block short (3091 x 5192 bf16 sigmoid 24.6 against 21.9 us, 512 x
+// 20000 fp32 backward 25.0 and 23.5).
 int64_t blocks_of(int64_t turns, int waves, int room) {
   const int64_t resident = (int64_t)kCus * (4 * room / waves);
-  return turns <= resident ? turns : ceil_div(turns, ceil_div(turns, resident));
+  return turns <= resident ? turns : resident;
 }
 
 bool act_ok(int act) { return act >= XDFM_ACT_IDENTITY && act <= XDFM_ACT_ELU; }
