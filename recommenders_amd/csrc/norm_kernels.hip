@@ -11,7 +11,7 @@
 //   1024 x 65536 fp32 relu, forward     91 us, 5.9 TB/s of 6.2 that a plain streaming addition reaches
 //    512 x 65536 fp32 relu, backward    73 us, 5.5 TB/s, 5 of them in the second launch that joins 256 partial sums
 //   2496 x 16384 bf16, backward         47.5 us, 5.2 TB/s, 5 of them in the second launch
-// Rows longer than the registers of 16 waves (16384 elements forward, 8192 backward) take a slower way (2.2 to 2.9 TB/s).
+// Rows of more than 16384 elements, which the registers of a block do not hold, take a slower way (2.2 to 2.9 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "xdfm_common.h"
@@ -575,27 +575,31 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
   }
 }
 
-// Rows of 2 to 5 pieces a lane, each in one wave, foremost of 16 bits: its sums need no barrier, and eight waves of up to 256
-// registers have more bytes under way (80 KB of a CU's reads at 5 pieces) than the sixteen that hold 8 elements a thread
-// (30 KB).  What is not needed all the time makes room for that: gamma and beta lie in LDS, xhat is formed again for dx.
-// 2496 x 16384 bf16 47.5 against 53.5 us, with tanh 59 and 74; 640 columns 16.7 and 21.3; 1024 rows of 2496 11.1 and 12.3,
-// 256 rows, where few CUs have a block, 9.5 and 8.9.  fp32, of which those have twice the bytes under way, gains less
-// (640 x 16384 23.2 and 25.3, 1280 x 4096 15.4 and 18.1) and loses where the pass does not stay in the caches (1280 x 65536
-// 182 and 170): 3 to 6 pieces there, and small passes only.
+// Rows in 1, 2, 4 or 8 waves (W) with up to 40 elements of 16 bits or 32 of fp32 a lane.  A block is eight waves of up to
+// 256 registers: they have more bytes under way (80 KB of a CU's reads at 5 pieces) than the sixteen of 8 elements a thread
+// (30 KB), and the sums of a row alone in its wave need no barrier.  What is not needed all the time makes room for that:
+// gamma and beta lie in LDS, xhat is formed again for dx.  us, against the kernel above (beyond 8192 columns: below):
+//   bf16   640 x 16384  16.7, 21.3    2496 x 16384  47.5, 53.5 (with tanh 59, 74)    4346 x 8192  48, 65    8192 x 8192  77, 78
+//          12288 x 8192  109, 269     16384 x 64  14.6, 16.7
+//   fp32   640 x 16384  23.2, 25.3    1280 x 4096  15.4, 18.1    1280 x 65536  182, 170    12288 x 8192  212, 460
 constexpr int kRowWaves = 8;
-template <typename T, int NV, int MODE, bool ACT>
+template <typename T, int W, int NV, int MODE, bool ACT>
 __global__ __launch_bounds__(64 * kRowWaves) void layer_norm_bwd_wave_kernel(
     const T* x, int64_t xs, const T* dy, int64_t dys, int64_t rows, int cols, const float* __restrict__ gamma,
     const float* __restrict__ beta, const float* __restrict__ stats, int act, T* dx, int64_t dxs,
     float* __restrict__ part_g, float* __restrict__ part_b) {
   constexpr int V = kVec<T>;
-  __shared__ u32x4 weights[2][NV][V / 4][64];
-  __shared__ float acc[2][kRowWaves][2 * V][64 + 64 / V];  // (read V apart: the padding spreads them over the banks)
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
-  const Pieces<T, NV> at(lane * V, 64 * V, cols);
+  constexpr int kGroups = kRowWaves / W;  // rows at once
+  __shared__ u32x4 weights[2][NV][V / 4][64 * W];
+  // (read V apart: the padding spreads them over the banks)
+  __shared__ float acc[kGroups > 1 ? 2 : 1][kGroups > 1 ? kRowWaves : 1][2 * V][64 + 64 / V];
+  __shared__ float sh[2][kMaxWaves][2];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), group = wave / W;
+  const int lane = (int)threadIdx.x - 64 * W * group;
+  const Pieces<T, NV> at(lane * V, 64 * W * V, cols);
 #pragma unroll
   for (int k = 0; k < NV; ++k)
-    if (wave == k) {
+    if (group == k % kGroups) {
 #pragma unroll
       for (int i = 0; i < V / 4; ++i) {
         weights[0][k][i][lane] = *reinterpret_cast<const u32x4_any*>(gamma + at.c[k] + 4 * i);
@@ -619,8 +623,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void layer_norm_bwd_wave_kernel(
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int j = 0; j < V; ++j) sg[k][j] = sb[k][j] = 0.f;
-  const int64_t stride = (int64_t)gridDim.x * kRowWaves;
-  int64_t r = (int64_t)blockIdx.x * kRowWaves + wave;
+  const int64_t stride = (int64_t)gridDim.x * kGroups;
+  int64_t r = (int64_t)blockIdx.x * kGroups + group;
   u32x4 xn[NV], dn[NV];
   float mean_n = 0.f, rstd_n = 0.f;
   const auto fetch = [&](int64_t row) {
@@ -633,7 +637,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void layer_norm_bwd_wave_kernel(
     rstd_n = stats[rows + row];
   };
   if (r < rows) fetch(r);
-  for (; r < rows; r += stride) {
+  int turn = 0;
+  // (waves that share rows meet at barriers: all of a block's take every turn, with or without a row)
+  for (; (W == 1 ? r : r - group) < rows; r += stride, turn ^= 1) {
+    const bool live = W == 1 || kGroups == 1 || r < rows;
     const float mean = mean_n, rstd = rstd_n;
     u32x4 xw[NV], dw[NV];
     float t[NV][V], s[2] = {0.f, 0.f};
@@ -646,35 +653,38 @@ __global__ __launch_bounds__(64 * kRowWaves) void layer_norm_bwd_wave_kernel(
       dw[k] = dn[k];
     }
     if (r + stride < rows) fetch(r + stride);  // the next row is under way while this one is worked on
+    if (live) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      __builtin_amdgcn_sched_barrier(0);
-      float xh[1][V], g[1][V], d[1][V];
-      unpack<T>(xw[k], xh[0]);
-      weight(0, k, l, g);
+      for (int k = 0; k < NV; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        float xh[1][V], g[1][V], d[1][V];
+        unpack<T>(xw[k], xh[0]);
+        weight(0, k, l, g);
 #pragma unroll
-      for (int j = 0; j < V; ++j) xh[0][j] = (xh[0][j] - mean) * rstd;
-      asm volatile("" : "+v"(dw[k]));
-      unpack<T>(dw[k], d[0]);
-      if (k == NV - 1) mask(d[0], at.skip[k]);
-      if constexpr (ACT) {
-        float b[1][V];
-        const u32x4 xk[1] = {xw[k]};
-        weight(1, k, l, b);
-        through_act<T>(d, xh, xk, g, b, mean, rstd, act);
+        for (int j = 0; j < V; ++j) xh[0][j] = (xh[0][j] - mean) * rstd;
+        asm volatile("" : "+v"(dw[k]));
+        unpack<T>(dw[k], d[0]);
+        if (k == NV - 1) mask(d[0], at.skip[k]);
+        if constexpr (ACT) {
+          float b[1][V];
+          const u32x4 xk[1] = {xw[k]};
+          weight(1, k, l, b);
+          through_act<T>(d, xh, xk, g, b, mean, rstd, act);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          sg[k][j] = fmaf(d[0][j], xh[0][j], sg[k][j]);
+          sb[k][j] += d[0][j];
+          asm volatile("" : "+v"(sg[k][j]), "+v"(sb[k][j]));
+          t[k][j] = d[0][j] * g[0][j];
+          s[0] += t[k][j];
+          s[1] = fmaf(t[k][j], xh[0][j], s[1]);
+        }
+        asm volatile("" : "+v"(s[0]), "+v"(s[1]));
       }
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        sg[k][j] = fmaf(d[0][j], xh[0][j], sg[k][j]);
-        sb[k][j] += d[0][j];
-        asm volatile("" : "+v"(sg[k][j]), "+v"(sb[k][j]));
-        t[k][j] = d[0][j] * g[0][j];
-        s[0] += t[k][j];
-        s[1] = fmaf(t[k][j], xh[0][j], s[1]);
-      }
-      asm volatile("" : "+v"(s[0]), "+v"(s[1]));
     }
-    row_sum<64, 2>(s, 1, nullptr);
+    row_sum<W == 1 ? 64 : 0>(s, W, sh[turn]);
+    if (!live) continue;
     const float a = -(s[0] / n) * rstd, b = -(s[1] / n) * rstd * rstd;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -691,25 +701,35 @@ __global__ __launch_bounds__(64 * kRowWaves) void layer_norm_bwd_wave_kernel(
         store_piece<MODE, T, V>(to, at.skip[k], t[k]);
     }
   }
-  // the waves' sums, a piece at a time through one of two buffers: [wave][sum][lane] -> one sum per column
+  if constexpr (kGroups == 1) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (at.skip[k] < V) {
+        store_piece<kPlain, float, V>(part_g + (int64_t)blockIdx.x * cols + at.c[k], at.skip[k], sg[k]);
+        store_piece<kPlain, float, V>(part_b + (int64_t)blockIdx.x * cols + at.c[k], at.skip[k], sb[k]);
+      }
+    return;
+  }
+  // the groups' sums, a piece at a time through one of two buffers: [wave][sum][lane] -> one sum per column
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      acc[k & 1][wave][j][lane] = sg[k][j];
-      acc[k & 1][wave][V + j][lane] = sb[k][j];
+      acc[k & 1][wave][j][lane & 63] = sg[k][j];
+      acc[k & 1][wave][V + j][lane & 63] = sb[k][j];
     }
     __syncthreads();
+    constexpr int kSums = V * 64 * W;  // of one kind; whole turns of the block
+    static_assert(2 * kSums % (64 * kRowWaves) == 0, "");
 #pragma unroll
-    for (int i = 0; i < 2 * V * 64; i += 64 * kRowWaves) {
+    for (int i = 0; i < 2 * kSums; i += 64 * kRowWaves) {
       const int e = i + (int)threadIdx.x;
-      if (e >= 2 * V * 64) break;
       // neighbours in a block take neighbouring columns of one of the two sums
-      const int which = e / (V * 64), rest = e % (V * 64), l = rest / V, j = rest % V;
-      const int at0 = l * V + k * 64 * V, c = min(at0, cols - V), skip = at0 - c;
+      const int which = e / kSums, l = e % kSums / V, j = e % V;
+      const int at0 = (k * 64 * W + l) * V, c = min(at0, cols - V), skip = at0 - c;
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kRowWaves; ++w) sum += acc[k & 1][w][which * V + j][l];
+      for (int q = 0; q < kGroups; ++q) sum += acc[k & 1][q * W + (l >> 6)][which * V + j][l & 63];
       if (j >= skip) (which ? part_b : part_g)[(int64_t)blockIdx.x * cols + c + j] = sum;
     }
   }
@@ -909,29 +929,47 @@ template <typename T, int MODE>
 int bwd_as(const void* x, int64_t xs, const void* dy, int64_t dys, int64_t rows, int cols, const float* gamma,
            const float* beta, const float* stats, int act, void* dx, int64_t dxs, float* dgamma, float* dbeta, float* ws,
            hipStream_t st) {
-  const int alone = (int)ceil_div(cols, 64 * kVec<T>);
-  constexpr bool kAlone = sizeof(T) == 2 || MODE == kPlain;
-  if (kAlone && alone >= (sizeof(T) == 2 ? 2 : 3) && alone <= (sizeof(T) == 2 ? 5 : 6) && ceil_div(rows, kRowWaves) >= kCus / 2) {
-    const int64_t blocks = blocks_of(ceil_div(rows, kRowWaves), kRowWaves, alone * kVec<T> <= (act == XDFM_ACT_IDENTITY ? 16 : 12) ? 4 : 2);
-    const auto go = [&](auto kernel) {
-      XDFM_LAUNCH("layer_norm_bwd_wave_kernel", st, kernel, dim3((unsigned)blocks), dim3(64 * kRowWaves), 0, (const T*)x,
-                  xs, (const T*)dy, dys, rows, cols, gamma, beta, stats, act, (T*)dx, dxs, ws, ws + blocks * cols);
-    };
-#define CASE(NV)                                                           \
-  if (alone == NV)                                                         \
-    go(act == XDFM_ACT_IDENTITY ? layer_norm_bwd_wave_kernel<T, NV, MODE, false> \
-                                : layer_norm_bwd_wave_kernel<T, NV, MODE, true>);
-    if constexpr (kAlone) {
-      CASE(3) CASE(4) CASE(5)
-      if constexpr (sizeof(T) == 2) {
-        CASE(2)
-      } else {
-        CASE(6)
-      }
-    }
-#undef CASE
+  // Rows in waves of many registers, see there, if they are enough to give most CUs a block (16-bit 2496 x 256 9.5 against
+  // 8.9 us, x 1024 11.1 and 12.3; four waves a row need two rounds: 8192 x 600 21 and 18, x 1024 20 and 19.6).  fp32, of
+  // which the other kernel has twice the bytes under way, only where the pass stays in the caches, or is too long for it.
+  const int need = (int)ceil_div(cols, 64 * kVec<T>);
+  const auto go = [&](auto kernel, int w, int each) {
+    const int64_t blocks = blocks_of(ceil_div(rows, kRowWaves / w), kRowWaves, each <= (act ? 12 : 16) ? 4 : 2);
+    XDFM_LAUNCH("layer_norm_bwd_wave_kernel", st, kernel, dim3((unsigned)blocks), dim3(64 * kRowWaves), 0, (const T*)x,
+                xs, (const T*)dy, dys, rows, cols, gamma, beta, stats, act, (T*)dx, dxs, ws, ws + blocks * cols);
     return (int)blocks;
+  };
+  const auto fits = [&](int w, int most) {
+    return need <= most * w && ceil_div(rows, kRowWaves / w) >= (w == 4 ? 2 * kCus : kCus / 2);
+  };
+#define CASE(W, NV)                                                               \
+  if (need <= W * NV)                                                             \
+    return go(act ? layer_norm_bwd_wave_kernel<T, W, NV, MODE, true>              \
+                  : layer_norm_bwd_wave_kernel<T, W, NV, MODE, false>, W, NV * kVec<T>);
+  static_assert(XDFM_ACT_IDENTITY == 0, "");
+  if constexpr (sizeof(T) == 2) {
+    if (need >= 2 && fits(1, 5)) {
+      CASE(1, 2) CASE(1, 3) CASE(1, 4) CASE(1, 5)
+    }
+    if (need > 5 && fits(2, 5)) {
+      CASE(2, 3) CASE(2, 4) CASE(2, 5)
+    }
+    if (need > 10 && fits(4, 5)) {
+      CASE(4, 3) CASE(4, 4) CASE(4, 5)
+    }
+    if (need > 16) {
+      CASE(8, 3) CASE(8, 4)
+    }
+  } else {
+    if constexpr (MODE == kPlain)
+      if (need >= 3 && fits(1, 6)) {
+        CASE(1, 3) CASE(1, 4) CASE(1, 5) CASE(1, 6)
+      }
+    if (need > 32) {
+      CASE(8, 5) CASE(8, 6) CASE(8, 7) CASE(8, 8)
+    }
   }
+#undef CASE
   // 8 elements a thread: with their weights and the weights' gradients they take 6 registers each
   constexpr int kWave = 8 / kVec<T>;
   const Shape s = shape_of(cols, kVec<T>, kWave, kWave);

@@ -188,9 +188,12 @@ def test_forward_and_backward_match_the_formula(rows, cols, kind):
 @pytest.mark.parametrize("rows,cols,pad,offset", [(1017, 513, 0, 0), (1031, 1000, 3, 1), (4099, 1024, 0, 0),
                                                   (1100, 1025, 5, 0), (1024, 1536, 8, 0), (2051, 1537, 0, 3),
                                                   (1500, 2041, 7, 1), (1019, 2048, 0, 0), (4101, 2049, 0, 1),
-                                                  (4096, 2496, 6, 0), (4200, 2560, 0, 0), (1500, 700, 1, 2)])
-def test_many_rows_of_one_wave_each(act, kind, rows, cols, pad, offset):
-    """2 to 6 pieces a lane: out of place, and in place with the same bits."""
+                                                  (4096, 2496, 6, 0), (4200, 2560, 0, 0), (1500, 700, 1, 2),
+                                                  (511, 2561, 1, 0), (1027, 4096, 0, 1), (700, 5113, 7, 2),
+                                                  (257, 5121, 0, 0), (263, 8192, 0, 0), (259, 10233, 3, 1),
+                                                  (7, 8200, 0, 0), (261, 12289, 1, 1), (300, 16384, 0, 0)])
+def test_many_rows_of_a_few_waves_each(act, kind, rows, cols, pad, offset):
+    """2 to 6 pieces a lane, 1 to 16 waves a row: out of place, and in place with the same bits."""
     dtype, code = TYPES[kind]
     x, dy, gamma, beta, view = make(rows, cols, dtype, seed=rows + cols, pad=pad, offset=offset)
     y, dx = view(torch.zeros_like(x)), view(torch.zeros_like(x))
