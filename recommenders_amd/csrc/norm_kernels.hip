@@ -11,7 +11,8 @@
 //   1024 x 65536 fp32 relu, forward     91 us, 5.9 TB/s of 6.2 that a plain streaming addition reaches
 //    512 x 65536 fp32 relu, backward    73 us, 5.5 TB/s, 5 of them in the second launch that joins 256 partial sums
 //   2496 x 16384 bf16, backward         47.5 us, 5.2 TB/s, 5 of them in the second launch
-// Rows of more than 16384 elements, which the registers of a block do not hold, take a slower way (2.2 to 2.9 TB/s).
+// Rows that the registers of a block do not hold (16384 elements backward; 18432, of 16 bits 20480, forward) take a slower
+// way (2.2 to 2.9 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "xdfm_common.h"
@@ -319,10 +320,12 @@ __device__ __forceinline__ void through_act(float (&d)[NV][V], const float (&xh)
 // row to row, and with them gamma and beta.  (Re-reading the row for each of the three sums instead, one block a row:
 // 226 against 91 us at 1024 x 65536 fp32.  gamma and beta by single elements instead of 16 bytes: 21 against 6 us at
 // 1001 x 4099 fp16, where most waves see one row.)
+// waves of a CU that hold `each` elements a lane (registers)
+constexpr int places(int each) { return each <= 16 ? 16 : each <= 24 ? 12 : 8; }
 // (Two pieces of 16 bits take 97 registers where five waves a SIMD leave 96 to each: asked for, 1001 x 4099 fp16 tanh 7.35
 // against 7.75 us, 1001 x 5000 7.8 and 9.3.)
 template <typename T, int G, int NV, int MODE>
-__global__ __launch_bounds__(G ? kThreads : 64 * kMaxWaves,
+__global__ __launch_bounds__(G ? kThreads : 64 * places(NV * kVec<T>),
                              G == 64 && NV == 2 && sizeof(T) == 2 ? 5 : 1) void layer_norm_fwd_kernel(
     const T* x, int64_t xs, int64_t rows, int cols, const float* __restrict__ gamma, const float* __restrict__ beta,
     float eps, int act, T* y, int64_t ys, float* __restrict__ stats) {
@@ -888,16 +891,26 @@ bool extent_ok(int64_t rows, int64_t stride, int cols) {
 template <typename T, int MODE>
 void fwd_as(const void* x, int64_t xs, int64_t rows, int cols, const float* gamma, const float* beta, float eps, int act,
          void* y, int64_t ys, float* stats, hipStream_t st) {
-  // 16 elements a thread; up to 24 where they hold the row without company (16384 x 1536 bf16 17.5 against 19.2 us, 1100
-  // columns 17.3 and 20.0; with 32 elements, 2048 columns, 29.2 and 24.7).  40 of 16 bits do better than three waves that
-  // a row fills by four fifths, if there are enough of them (2496 x 16384 bf16 30.8 and 32.2 us, with tanh 42 and 53;
-  // 1024 rows 5.4 and 4.9).
-  constexpr int kWave = 16 / kVec<T>, kMore = 40 / kVec<T>;
-  Shape s = shape_of(cols, kVec<T>, 24 / kVec<T>, kWave);
-  if (sizeof(T) == 2 && rows >= 4096 && ceil_div(cols, 64 * kVec<T>) == kMore) s = {64, kMore, 1};
+  // 16 elements a thread, up to 24 where they hold the row without company (1536 x 16384 bf16 17.5 against 19.2 us, 1100
+  // columns 17.3 and 20.0).  Many longer rows of 16 bits, and rows too long for 16: 16, 24 or 40 elements a thread,
+  // whichever leaves the fewest of a CU's lanes empty, in the row and behind the last row that fits (2496 x 16384 bf16 31.0
+  // against 32.3 us; 10240 x 5192 38.7 and 50.4; 6144 x 16384 sigmoid 81 and 110; 18000 x 5192 75 and 117, fp32 138 and 210;
+  // but 9000 x 300 7.1 and 6.0, fp32 9000 x 5192 68.5 and 65).
+  constexpr int kWave = 16 / kVec<T>, kMore = 24 / kVec<T>, kMost = 40 / kVec<T>;
+  Shape s = shape_of(cols, kVec<T>, kMore, kWave);
+  const int64_t need = ceil_div(cols, 64 * kVec<T>);
+  if (s.pieces == 0 || (sizeof(T) == 2 && need > kMore && rows >= 4096)) {
+    double best = 0.;
+    for (const int each : {kWave, kMore, kMost}) {
+      const int64_t at = places(each * kVec<T>), waves = ceil_div(need, each);
+      const double filled = (double)(need * (at / waves)) / (double)(each * at);  // 0: the row does not fit
+      if (filled > best && (sizeof(T) == 2 || each != kMost)) best = filled, s = {waves == 1 ? 64 : 0, each, (int)waves};
+    }
+  }
   const dim3 block(s.group ? kThreads : 64 * s.waves);
   const int64_t turns = s.group ? ceil_div(rows, kThreads / s.group) : rows;
-  const int each = s.pieces * kVec<T>, room = each > 24 ? 2 : each > 16 ? 3 : each > 8 ? (sizeof(T) == 2 && s.group ? 5 : 4) : each ? 7 : 8;
+  const int each = s.pieces * kVec<T>;
+  const int room = each > 16 ? places(each) / 4 : each > 8 ? (sizeof(T) == 2 && s.group ? 5 : 4) : each ? 7 : 8;
   const dim3 grid((unsigned)blocks_of(turns, (int)block.x / 64, room));
 #define CASE(G, NV)                                                                                              \
   if (s.group == G && s.pieces == NV) {                                                                          \
@@ -907,9 +920,9 @@ void fwd_as(const void* x, int64_t xs, int64_t rows, int cols, const float* gamm
   }
   CASE(8, 1) CASE(16, 1) CASE(32, 1) CASE(64, 1) CASE(64, 2)
   if constexpr (kWave == 4) {
-    CASE(64, 3) CASE(64, 4) CASE(64, 5) CASE(64, 6) CASE(0, 4)
+    CASE(64, 3) CASE(64, 4) CASE(64, 5) CASE(64, kMore) CASE(0, kWave) CASE(0, kMore)
   } else {
-    CASE(64, 3) CASE(64, kMore) CASE(0, 2)
+    CASE(64, kMore) CASE(64, kMost) CASE(0, kWave) CASE(0, kMore) CASE(0, kMost)
   }
 #undef CASE
   XDFM_LAUNCH("layer_norm_fwd_long_kernel", st, layer_norm_fwd_long_kernel<T>, grid, block, 0, (const T*)x, xs, rows,

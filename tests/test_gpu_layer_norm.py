@@ -191,7 +191,9 @@ def test_forward_and_backward_match_the_formula(rows, cols, kind):
                                                   (4096, 2496, 6, 0), (4200, 2560, 0, 0), (1500, 700, 1, 2),
                                                   (511, 2561, 1, 0), (1027, 4096, 0, 1), (700, 5113, 7, 2),
                                                   (257, 5121, 0, 0), (263, 8192, 0, 0), (259, 10233, 3, 1),
-                                                  (7, 8200, 0, 0), (261, 12289, 1, 1), (300, 16384, 0, 0)])
+                                                  (7, 8200, 0, 0), (261, 12289, 1, 1), (300, 16384, 0, 0),
+                                                  (4097, 2700, 1, 1), (4099, 5119, 0, 0), (5, 18432, 0, 0),
+                                                  (9, 20479, 1, 1), (3, 20481, 0, 0)])
 def test_many_rows_of_a_few_waves_each(act, kind, rows, cols, pad, offset):
     """2 to 6 pieces a lane, 1 to 16 waves a row: out of place, and in place with the same bits."""
     dtype, code = TYPES[kind]
