@@ -237,9 +237,32 @@ __device__ __forceinline__ float expm1_of(float u) {
   return u > -0.5f ? fmaf(u * u, q, u) : __builtin_amdgcn_exp2f(1.44269504f * u) - 1.f;
 }
 
+// Where a result is stored in 16 bits, and for slopes there, the exponent's own rounding may stay: |u| 2^-24 of the value,
+// 2^-17 at most before the value itself is out of range, a hundredth of the storage's half step and less; a slope is off
+// by less than 2^-24 so (|u| e^-|u| < 0.4).  Half the operations of a sigmoid: 632 x 12980 bf16 11.9 against 14.4 us.
+__device__ __forceinline__ float exp_quick(float u) { return __builtin_amdgcn_exp2f(u * 1.44269504f); }
+__device__ __forceinline__ float sigmoid_quick(float u) { return __builtin_amdgcn_rcpf(1.f + exp_quick(-u)); }
+// (up to 0.1 the series, to 2^-23 and 2^-20; from there on 2^-22 of 1 is 2^-18 of the value, a sixtieth of fp16's half
+// step.  Tanh 409 x 54188 bf16 29.2 against 32.0 us.)
+__device__ __forceinline__ float tanh_16(float u) {
+  const float w = u * u;
+  const float small = fmaf(u * w, fmaf(w, 0.133333333f, -0.333333333f), u);
+  const float large = copysignf(fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.88539008f * fabsf(u)) + 1.f), 1.f), u);
+  return fabsf(u) < 0.1f ? small : large;
+}
+__device__ __forceinline__ float expm1_16(float u) {
+  const float small = fmaf(u * u, fmaf(u, fmaf(u, 0.0416666667f, 0.166666667f), 0.5f), u);
+  return u > -0.1f ? small : exp_quick(u) - 1.f;
+}
+// tanh |u|, off by 2^-22 at most: near 0 only a slope can bear that
+__device__ __forceinline__ float tanh_quick(float u) {
+  return fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.88539008f * fabsf(u)) + 1.f), 1.f);
+}
+
 // v <- act(v).  (One switch for all of a thread's elements: the cases are straight code.)
-template <int NV, int V>
+template <typename T, int NV, int V>
 __device__ __forceinline__ void activate_all(float (&v)[NV][V], int act) {
+  constexpr bool kQuick = sizeof(T) == 2;
 #define XDFM_EACH(EXPR)              \
   _Pragma("unroll") for (int k = 0; k < NV; ++k) _Pragma("unroll") for (int j = 0; j < V; ++j) { \
     const float u = v[k][j];         \
@@ -248,34 +271,22 @@ __device__ __forceinline__ void activate_all(float (&v)[NV][V], int act) {
   break;
   switch (act) {
     case XDFM_ACT_RELU: XDFM_EACH(u > 0.f ? u : 0.f)
-    case XDFM_ACT_SIGMOID: XDFM_EACH(sigmoid_of(u))
-    case XDFM_ACT_TANH: XDFM_EACH(tanh_of(u))
-    case XDFM_ACT_ELU: XDFM_EACH(u > 0.f ? u : expm1_of(u))
+    case XDFM_ACT_SIGMOID: XDFM_EACH(kQuick ? sigmoid_quick(u) : sigmoid_of(u))
+    case XDFM_ACT_TANH: XDFM_EACH(kQuick ? tanh_16(u) : tanh_of(u))
+    case XDFM_ACT_ELU: XDFM_EACH(u > 0.f ? u : kQuick ? expm1_16(u) : expm1_of(u))
     default: break;
   }
 #undef XDFM_EACH
 }
 
-// act'(u) for one element, from 64 bits for relu: 32 bits lose the sign of u where gamma xhat and beta nearly cancel
+// The slope of relu, from 64 bits: 32 bits lose the sign of u where gamma xhat and beta nearly cancel
 // (three roundings of 2^-24 of |beta|: near_zero)
 __device__ __forceinline__ bool near_zero(float u, float b) { return fabsf(u) <= 6e-7f * fabsf(b); }
 __device__ __forceinline__ float on_exactly(float x, float mean, float rstd, float g, float b) {
   return ((double)x - (double)mean) * (double)rstd * (double)g + (double)b > 0.0 ? 1.f : 0.f;
 }
-__device__ __forceinline__ float slope(float u, int act, float x, float mean, float rstd, float g, float b) {
-  switch (act) {
-    case XDFM_ACT_RELU: return near_zero(u, b) ? on_exactly(x, mean, rstd, g, b) : u > 0.f ? 1.f : 0.f;
-    case XDFM_ACT_SIGMOID: {
-      const float s = sigmoid_of(u);
-      return s * (1.f - s);
-    }
-    case XDFM_ACT_TANH: {
-      const float t = tanh_of(u);
-      return 1.f - t * t;
-    }
-    case XDFM_ACT_ELU: return u > 0.f ? 1.f : exp_of(u);
-    default: return 1.f;
-  }
+__device__ __forceinline__ float relu_slope(float u, float x, float mean, float rstd, float g, float b) {
+  return near_zero(u, b) ? on_exactly(x, mean, rstd, g, b) : u > 0.f ? 1.f : 0.f;
 }
 
 // d <- d act'(gamma xhat + beta) for all of a thread's elements; x: the raw pieces of the row
@@ -283,6 +294,7 @@ template <typename T, int NV, int V>
 __device__ __forceinline__ void through_act(float (&d)[NV][V], const float (&xh)[NV][V], const u32x4 (&x)[NV],
                                             const float (&g)[NV][V], const float (&b)[NV][V], float mean, float rstd,
                                             int act) {
+  constexpr bool kQuick = sizeof(T) == 2;
 #define XDFM_EACH(EXPR)                              \
   _Pragma("unroll") for (int k = 0; k < NV; ++k) _Pragma("unroll") for (int j = 0; j < V; ++j) { \
     const float u = xh[k][j] * g[k][j] + b[k][j];    \
@@ -299,29 +311,30 @@ __device__ __forceinline__ void through_act(float (&d)[NV][V], const float (&xh)
           unpack<T>(x[k], xv);
 #pragma unroll
           for (int j = 0; j < V; ++j)
-            d[k][j] *= slope(xh[k][j] * g[k][j] + b[k][j], XDFM_ACT_RELU, xv[j], mean, rstd, g[k][j], b[k][j]);
+            d[k][j] *= relu_slope(xh[k][j] * g[k][j] + b[k][j], xv[j], mean, rstd, g[k][j], b[k][j]);
         }
       } else {
         XDFM_EACH(d[k][j] *= u > 0.f ? 1.f : 0.f)
       }
       break;
     }
-    case XDFM_ACT_SIGMOID: XDFM_EACH(const float s = sigmoid_of(u); d[k][j] *= s * (1.f - s)) break;
-    case XDFM_ACT_TANH: XDFM_EACH(const float t = tanh_of(u); d[k][j] *= 1.f - t * t) break;
-    case XDFM_ACT_ELU: XDFM_EACH(d[k][j] *= u > 0.f ? 1.f : exp_of(u)) break;
+    case XDFM_ACT_SIGMOID: XDFM_EACH(const float s = kQuick ? sigmoid_quick(u) : sigmoid_of(u); d[k][j] *= s * (1.f - s)) break;
+    case XDFM_ACT_TANH: XDFM_EACH(const float t = kQuick ? tanh_quick(u) : tanh_of(u); d[k][j] *= 1.f - t * t) break;
+    case XDFM_ACT_ELU: XDFM_EACH(d[k][j] *= u > 0.f ? 1.f : kQuick ? exp_quick(u) : exp_of(u)) break;
     default: break;
   }
 #undef XDFM_EACH
 }
 
 // ------------------------------------------------------------------ forward
+// waves of a CU that hold `each` elements a lane (by their registers)
+constexpr int places(int each) { return each <= 16 ? 16 : each <= 24 ? 12 : 8; }
+
 // One pass over the data: a row lies in the registers of its G lanes (or of the block's threads) from the load to the
 // store, so the variance is taken around the mean and not from the sum of squares.  A thread keeps its columns from
 // row to row, and with them gamma and beta.  (Re-reading the row for each of the three sums instead, one block a row:
 // 226 against 91 us at 1024 x 65536 fp32.  gamma and beta by single elements instead of 16 bytes: 21 against 6 us at
 // 1001 x 4099 fp16, where most waves see one row.)
-// waves of a CU that hold `each` elements a lane (registers)
-constexpr int places(int each) { return each <= 16 ? 16 : each <= 24 ? 12 : 8; }
 // (Two pieces of 16 bits take 97 registers where five waves a SIMD leave 96 to each: asked for, 1001 x 4099 fp16 tanh 7.35
 // against 7.75 us, 1001 x 5000 7.8 and 9.3.)
 template <typename T, int G, int NV, int MODE>
@@ -381,7 +394,7 @@ __global__ __launch_bounds__(G ? kThreads : 64 * places(NV * kVec<T>),
     for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) v[k][j] = v[k][j] * rstd * g[k][j] + b[k][j];
-    activate_all(v, act);
+    activate_all<T>(v, act);
     if (r < rows) {
 #pragma unroll
       for (int k = 0; k < NV; ++k)
@@ -437,7 +450,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_fwd_long_kernel(
       load_weights<T, 1>(beta, at, false, b);
 #pragma unroll
       for (int j = 0; j < V; ++j) v[0][j] = (v[0][j] - mean) * rstd * g[0][j] + b[0][j];
-      activate_all(v, act);
+      activate_all<T>(v, act);
       store_piece<kPlain, T, V>(y + r * ys + at.c[0], at.skip[0], v[0]);
     }
     if (stats && threadIdx.x == 0) {
