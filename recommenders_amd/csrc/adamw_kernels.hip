@@ -542,9 +542,9 @@ extern "C" int xdfm_adamw_plan(const xdfm_adamw_tensor* tensors, int32_t n_tenso
   XDFM_REQUIRE(state_bits == 32 || state_bits == 8, "xdfm_adamw_plan: states have 32 or 8 bits, not %d", state_bits);
   XDFM_REQUIRE(((uintptr_t)image & 7) == 0, "xdfm_adamw_plan: misaligned image");
   try {
-    const int rc = make_plan(tensors, n_tensors, state_bits, nullptr, info);
-    if (rc) return rc;
-    if (!image) return check_apart(tensors, n_tensors, state_bits);
+    int rc = make_plan(tensors, n_tensors, state_bits, nullptr, info);
+    if (!rc) rc = check_apart(tensors, n_tensors, state_bits);
+    if (rc || !image) return rc;
     if (image_bytes < (size_t)info->bytes)
       return xdfm::fail(XDFM_E_WORKSPACE, "xdfm_adamw_plan: the image takes %lld bytes", (long long)info->bytes);
     return make_plan(tensors, n_tensors, state_bits, (Chunk*)image, info);
