@@ -422,8 +422,9 @@ typedef struct xdfm_adamw_args {
 
 /* Host only.  image = NULL: fills *info alone.  Otherwise `image` (host, 8-byte aligned, image_bytes >= the
  * info->bytes of a call without it) receives the plan and *info is filled again.  Refused, by either call and before
- * the image is written: null pointers of tensors with elements, misaligned fp32 / 16-bit pointers, and tensors of
- * which one is written where another one is written or read. */
+ * the image is written: null pointers of tensors with elements, misaligned fp32 / 16-bit pointers, tensors of which
+ * one is written where another one is written or read, and more than 2^24 - 1 chunks (of info->chunk_elems elements of
+ * one tensor at most: 3.4e10 elements in few tensors). */
 int xdfm_adamw_plan(const xdfm_adamw_tensor* tensors, int32_t n_tensors, int32_t state_bits, void* image,
                     size_t image_bytes, xdfm_adamw_plan_info* info);
 /* One step of all tensors.  plan: the image in device memory (8-byte aligned), info: as xdfm_adamw_plan gave it. */

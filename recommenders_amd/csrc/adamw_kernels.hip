@@ -30,6 +30,8 @@ constexpr int kBlock = 64;  // elements that share a scale
 // Elements of a chunk, two pieces of a thread: 40 bytes of record for 32 KB and more.  8-bit table with read-out 98 us,
 // with 4096 elements 100, with 8192 105; the wide model 28.9, 28.8, 31.0.
 constexpr int kChunk = 2048;
+// of a plan: a launch takes fewer than 2^32 threads
+constexpr int64_t kMostChunks = ((int64_t)1 << 32) / kThreads - 1;
 constexpr int kScaleMin = 48;  // units stay normal floats: 2^(48 - 159)
 constexpr uint32_t kMul1 = 0x9E3779B1u;  // 2^32 / golden ratio
 constexpr uint32_t kMul2 = 0x6A09E667u;  // the fraction of sqrt(2)
@@ -514,7 +516,8 @@ int make_plan(const xdfm_adamw_tensor* t, int n, int bits, Chunk* image, xdfm_ad
       c.gtype = x.grad_dtype;
     }
     out += x.n;
-    XDFM_REQUIRE(chunks < (int64_t)1 << 31, "xdfm_adamw_plan: too many elements");
+    XDFM_REQUIRE(chunks <= kMostChunks, "xdfm_adamw_plan: too many elements (more than %lld chunks of %d)",
+                 (long long)kMostChunks, kChunk);
   }
   info->bytes = chunks * (int64_t)sizeof(Chunk);
   info->chunks = chunks;
@@ -527,7 +530,7 @@ int make_plan(const xdfm_adamw_tensor* t, int n, int bits, Chunk* image, xdfm_ad
 int check_plan(const char* who, const void* plan, const xdfm_adamw_plan_info* info) {
   XDFM_REQUIRE(info, "%s: null argument", who);
   XDFM_REQUIRE((info->state_bits == 32 || info->state_bits == 8) && info->chunk_elems == kChunk && info->chunks >= 0 &&
-                   info->chunks < (int64_t)1 << 31 && info->bytes == info->chunks * (int64_t)sizeof(Chunk),
+                   info->chunks <= kMostChunks && info->bytes == info->chunks * (int64_t)sizeof(Chunk),
                "%s: *info is not what xdfm_adamw_plan gave", who);
   XDFM_REQUIRE(info->chunks == 0 || plan, "%s: null argument", who);
   XDFM_REQUIRE(((uintptr_t)plan & 7) == 0, "%s: misaligned plan", who);

@@ -42,3 +42,26 @@ def test_overlaps_are_refused_where_the_image_is_written_too(kw, bits, text):
     assert list(image) == [7] * (info.bytes // 8)
     assert plan([tensor(**apart)], bits, ctypes.addressof(image), info.bytes)[0] == 0
     assert list(image)[0] == 1 << 20
+
+
+def far(n):
+    """A tensor of n elements whose arrays lie 2^44 bytes apart."""
+    return tensor(param=1 << 44, grad=2 << 44, slot_m=3 << 44, slot_v=4 << 44, n=n)
+
+
+def test_a_plan_of_more_chunks_than_a_launch_takes_is_refused():
+    """256 threads a chunk, and a launch takes fewer than 2^32 threads: 2^24 - 1 chunks."""
+    _, info = plan([far(1)])
+    most = ((1 << 24) - 1) * info.chunk_elems
+    rc, info = plan([far(most)])
+    assert rc == 0 and info.chunks == (1 << 24) - 1 and info.elements == most
+    refused(plan([far(most + 1)])[0], "too many")
+    # in several tensors too
+    half = (1 << 23) * info.chunk_elems
+    second = tensor(param=5 << 44, grad=6 << 44, slot_m=7 << 44, slot_v=8 << 44, n=half)
+    refused(plan([far(half), second])[0], "too many")
+    # and a step does not take such an *info from elsewhere
+    more = _lib.AdamWPlanInfo((info.chunks + 1) * (info.bytes // info.chunks), info.chunks + 1, info.elements, 32,
+                              info.chunk_elems)
+    args = _lib.AdamWArgs(0.1, 0.9, 0.999, 1e-8, None, 1, 0)
+    refused(lib.xdfm_adamw_step(4096, ctypes.byref(more), ctypes.byref(args), None), "not what xdfm_adamw_plan gave")
