@@ -414,7 +414,7 @@ typedef struct xdfm_adamw_plan_info {
 } xdfm_adamw_plan_info;
 
 typedef struct xdfm_adamw_args {
-  double lr, beta1, beta2, eps; /* betas in [0, 1), eps in [1e-30, 1e30] */
+  double lr, beta1, beta2, eps; /* lr in [0, 1e20], betas in [0, 1), eps in [1e-30, 1e30] */
   const float* opt_state; /* NULL, or device: t = max(opt_state[3], 1) (xdfm_opt_advance): a step can be captured */
   int64_t step;           /* t, 1 for the first step; used where opt_state is NULL */
   uint64_t seed;          /* of the rounding of 8-bit states */

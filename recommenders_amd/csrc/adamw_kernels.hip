@@ -561,7 +561,8 @@ extern "C" int xdfm_adamw_step(const void* plan, const xdfm_adamw_plan_info* inf
   const int rc = check_plan("xdfm_adamw_step", plan, info);
   if (rc) return rc;
   XDFM_REQUIRE(args, "xdfm_adamw_step: null argument");
-  XDFM_REQUIRE(std::isfinite(args->lr) && args->lr >= 0, "xdfm_adamw_step: lr has to be finite and not negative");
+  // (lr / (1 - beta1^t) stays finite in 32 bits: 1 - beta1 is 2^-53 at least)
+  XDFM_REQUIRE(args->lr >= 0 && args->lr <= 1e20, "xdfm_adamw_step: lr has to lie in [0, 1e20]");
   XDFM_REQUIRE(args->beta1 >= 0 && args->beta1 < 1 && args->beta2 >= 0 && args->beta2 < 1,
                "xdfm_adamw_step: beta1 and beta2 have to lie in [0, 1)");
   XDFM_REQUIRE(args->eps >= 1e-30 && args->eps <= 1e30, "xdfm_adamw_step: eps has to lie in [1e-30, 1e30]");

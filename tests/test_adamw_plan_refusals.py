@@ -65,3 +65,11 @@ def test_a_plan_of_more_chunks_than_a_launch_takes_is_refused():
                               info.chunk_elems)
     args = _lib.AdamWArgs(0.1, 0.9, 0.999, 1e-8, None, 1, 0)
     refused(lib.xdfm_adamw_step(4096, ctypes.byref(more), ctypes.byref(args), None), "not what xdfm_adamw_plan gave")
+
+
+def test_a_rate_beyond_what_32_bits_hold_is_refused():
+    """lr / (1 - beta1^t) is formed in 32 bits: infinite, it would make NaN of every parameter whose m is 0."""
+    _, info = plan([tensor()])
+    for lr in (1e39, 3e38, 1.1e20):
+        args = _lib.AdamWArgs(lr, 0.9, 0.999, 1e-8, None, 1, 0)
+        refused(lib.xdfm_adamw_step(4096, ctypes.byref(info), ctypes.byref(args), None), "lr has to lie in")
