@@ -77,6 +77,8 @@ _TYPED_KEYS = (
         ).split(),
     ),
     (list, "list", "layer_sizes activation dropout att_fcn_layer_sizes dilations".split()),
+    # (no counterpart in the reference: the model asks for `is True`, and a 1 would silently leave the norm out)
+    (bool, "bool", ["enable_LN"]),
 )
 
 

@@ -61,7 +61,10 @@ LN_EPS = 1e-5
 
 def layer_norm_on(hp):
     """enable_LN (no counterpart in the reference): a layer norm behind every product of the DNN tower."""
-    return hp.values().get("enable_LN", False) is True
+    on = hp.values().get("enable_LN", False)
+    if not isinstance(on, bool):
+        raise TypeError("Parameters enable_LN must be bool")
+    return on
 
 
 def bn_state_shapes(hp):
