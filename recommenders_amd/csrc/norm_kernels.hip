@@ -15,6 +15,8 @@
 // way (2.2 to 2.9 TB/s).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "xdfm_common.h"
 
 namespace {
@@ -833,27 +835,33 @@ __global__ __launch_bounds__(kThreads) void layer_norm_bwd_long_sums_kernel(
   store_piece<kPlain, float, V>(part + (int64_t)(parts + p) * cols + at.c[0], at.skip[0], sb);
 }
 
-// dgamma (blockIdx.y = 0) and dbeta from the blocks' partial sums: 32 columns by 32 slices of the parts per block
+// dgamma (blockIdx.y = 0) and dbeta from the blocks' partial sums: 32 columns by 32 slices of the parts per block.  Blocks
+// walk the columns: a launch takes fewer than 2^32 threads, which 2^27 columns would need.
 constexpr int kFinish = 32;
+constexpr int kFinishBlocks = 1 << 16;  // (2^21 columns in one turn)
 __global__ __launch_bounds__(kFinish* kFinish) void layer_norm_bwd_finish_kernel(const float* __restrict__ part,
                                                                                  int parts, int cols,
                                                                                  float* __restrict__ dgamma,
                                                                                  float* __restrict__ dbeta) {
   __shared__ float sh[kFinish][kFinish + 1];
-  const int c = blockIdx.x * kFinish + threadIdx.x, slice = threadIdx.y;
+  const int slice = threadIdx.y;
   const float* p = part + (int64_t)blockIdx.y * parts * cols;
-  float s = 0.f;
-  if (c < cols) {
+  for (int64_t c0 = (int64_t)blockIdx.x * kFinish; c0 < cols; c0 += (int64_t)gridDim.x * kFinish) {
+    const int64_t c = c0 + threadIdx.x;
+    float s = 0.f;
+    if (c < cols) {
 #pragma unroll 8
-    for (int k = slice; k < parts; k += kFinish) s += p[(int64_t)k * cols + c];
-  }
-  sh[slice][threadIdx.x] = s;
-  __syncthreads();
-  if (slice == 0 && c < cols) {
-    s = 0.f;
+      for (int k = slice; k < parts; k += kFinish) s += p[(int64_t)k * cols + c];
+    }
+    sh[slice][threadIdx.x] = s;
+    __syncthreads();
+    if (slice == 0 && c < cols) {
+      s = 0.f;
 #pragma unroll
-    for (int k = 0; k < kFinish; ++k) s += sh[k][threadIdx.x];
-    (blockIdx.y ? dbeta : dgamma)[c] = s;
+      for (int k = 0; k < kFinish; ++k) s += sh[k][threadIdx.x];
+      (blockIdx.y ? dbeta : dgamma)[c] = s;
+    }
+    __syncthreads();
   }
 }
 
@@ -1109,8 +1117,8 @@ extern "C" int xdfm_layer_norm_bwd(const void* x, int64_t x_stride, const void* 
                           workspace, st);
   if (parts || rows == 0)
     XDFM_LAUNCH("layer_norm_bwd_finish_kernel", st, layer_norm_bwd_finish_kernel,
-                dim3((unsigned)ceil_div(cols, kFinish), 2), dim3(kFinish, kFinish), 0, workspace, parts, cols, dgamma,
-                dbeta);
+                dim3((unsigned)std::min<int64_t>(ceil_div(cols, kFinish), kFinishBlocks), 2), dim3(kFinish, kFinish), 0,
+                workspace, parts, cols, dgamma, dbeta);
   XDFM_LAUNCH_CHECK();
   return XDFM_OK;
 }
