@@ -409,7 +409,8 @@ __global__ __launch_bounds__(G ? kThreads : 64 * places(NV * kVec<T>),
   }
 }
 
-// Rows that the registers of a block do not hold: three passes over the row, which the caches serve.
+// Rows that the registers of a block do not hold: three passes over the row, which the caches serve.  The pieces' sums
+// are added up in 64 bits: a thread has up to 2^18 of them, and equal terms would round the same way every time.
 template <typename T>
 __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_fwd_long_kernel(
     const T* x, int64_t xs, int64_t rows, int cols, const float* __restrict__ gamma, const float* __restrict__ beta,
@@ -426,23 +427,31 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_fwd_long_kernel(
       unpack<T>(w[0], v[0]);
       return at;
     };
-    float s[1] = {0.f}, q[1] = {0.f}, v[1][V];
+    float v[1][V];
+    double sum = 0.;
     for (int c = c0; c < cols; c += step) {
       const Pieces<T, 1> at = piece(c, v);
       mask(v[0], at.skip[0]);
+      float p = 0.f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[0] += v[0][j];
+      for (int j = 0; j < V; ++j) p += v[0][j];
+      sum += p;
     }
+    float s[1] = {(float)sum};
     waves_sum(s, waves, sh[0]);
     const float mean = s[0] / n;
+    sum = 0.;
     for (int c = c0; c < cols; c += step) {
       const Pieces<T, 1> at = piece(c, v);
 #pragma unroll
       for (int j = 0; j < V; ++j) v[0][j] -= mean;
       mask(v[0], at.skip[0]);
+      float p = 0.f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) q[0] = fmaf(v[0][j], v[0][j], q[0]);
+      for (int j = 0; j < V; ++j) p = fmaf(v[0][j], v[0][j], p);
+      sum += p;
     }
+    float q[1] = {(float)sum};
     waves_sum(q, waves, sh[1]);
     const float rstd = 1.f / sqrtf(q[0] / n + eps);
     for (int c = c0; c < cols; c += step) {
@@ -789,16 +798,20 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_long_kernel(
   int turn = 0;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x, turn ^= 1) {
     const float mean = stats[r], rstd = stats[rows + r];
-    float s[2] = {0.f, 0.f};
+    double sum = 0., across = 0.;  // (see the forward kernel)
     for (int c = c0; c < cols; c += step) {
       const LongPiece<T> p(x + r * xs, dy + r * dys, gamma, beta, mean, rstd, act, c, cols);
+      float a = 0.f, b = 0.f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float t = p.t[0][j] * p.g[0][j];
-        s[0] += t;
-        s[1] = fmaf(t, p.xh[0][j], s[1]);
+        a += t;
+        b = fmaf(t, p.xh[0][j], b);
       }
+      sum += a;
+      across += b;
     }
+    float s[2] = {(float)sum, (float)across};
     waves_sum(s, waves, sh[turn]);
     const float ma = s[0] / n, mq = s[1] / n;
     for (int c = c0; c < cols; c += step) {
