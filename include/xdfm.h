@@ -788,6 +788,7 @@ int xdfm_bn_bwd_apply(const float* x, const float* y, const float* dy, int64_t B
  *     between consecutive rows, any alignment of the type; what lies between rows is neither read nor
  *     written.  gamma, beta, dgamma, dbeta [cols] and stats are fp32, as is all arithmetic.
  *   stats [2, rows] (NULL ok): mean, then rstd, for the backward pass.
+ * A row that holds a NaN or an infinity has no statistics: its y is NaN throughout, under relu too.
  * y may be x (same address and stride); dx may be dy or x.
  * Backward, from x and stats (y is not read):  du = dy * act'(u), u = gamma * xhat + beta (relu: on where u is
  * positive exactly);  t = du * gamma;  dx = rstd * (t - mean_row(t) - xhat * mean_row(t * xhat));

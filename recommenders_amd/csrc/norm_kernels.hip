@@ -272,7 +272,7 @@ __device__ __forceinline__ void activate_all(float (&v)[NV][V], int act) {
   }                                  \
   break;
   switch (act) {
-    case XDFM_ACT_RELU: XDFM_EACH(u > 0.f ? u : 0.f)
+    case XDFM_ACT_RELU: XDFM_EACH(u <= 0.f ? 0.f : u)  // (NaN stays: a row without statistics is no row of zeros)
     case XDFM_ACT_SIGMOID: XDFM_EACH(kQuick ? sigmoid_quick(u) : sigmoid_of(u))
     case XDFM_ACT_TANH: XDFM_EACH(kQuick ? tanh_16(u) : tanh_of(u))
     case XDFM_ACT_ELU: XDFM_EACH(u > 0.f ? u : kQuick ? expm1_16(u) : expm1_of(u))
