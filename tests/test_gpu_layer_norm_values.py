@@ -28,3 +28,22 @@ def test_a_row_that_is_not_finite_reads_as_nan_under_every_activation(act, kind,
         assert torch.isnan(y2[1]).all()
         keep = [r for r in range(rows) if r != 1]
         assert torch.equal(y2[keep], y[keep])
+
+
+def test_the_join_of_partial_sums_does_not_lose_small_ones():
+    """8192 x 20: a row's dy of 1 and 31 of 2^-24 in rows 64, 128, ..., which lie in partial sums of their own.  Half a
+    step under 1 each, they are lost where all 32 are added to the 1 one after the other: 31 u.  In a tree the 1 passes 5
+    additions of the join, and before it 7 within a block (8 groups of a wave, 8 waves and its own row) and 3 of the 4
+    parts of a slice: 15 u of 1 at most, and the small ones' own additions are exact."""
+    rows, cols = 8192, 20
+    x = torch.zeros((rows, cols), device="cuda")
+    dy = torch.zeros((rows, cols), device="cuda")
+    dy[0] = 1
+    dy[64:2048:64] = 2.0 ** -24
+    one, zero = torch.ones(cols, device="cuda"), torch.zeros(cols, device="cuda")
+    stats = torch.zeros((2, rows), device="cuda")
+    stats[0], stats[1] = -1, 1  # xhat = 1: dgamma is the same sum
+    dg, db = bwd(x, dy, 0, one, zero, stats, "identity", torch.empty_like(x))
+    exp = 1 + 31 * 2.0 ** -24
+    for got in (dg, db):
+        assert ((got.double() - exp).abs() <= 15 * U).all(), float((got.double() - exp).abs().max()) / U
