@@ -1,0 +1,93 @@
+"""AdamW steps of so many elements that their loads and stores go past the caches (256 MB and more): every type of
+gradient, tensors at odd addresses, chunks that end inside a tensor.
+
+m and v are equal to two products and their sum in fp32 in every bit; codes and scales to the definition's; p within
+test_gpu_adamw's bound.
+"""
+import numpy as np
+import pytest
+import torch
+
+from recommenders_amd.models.deeprec.models.adamw import AdamW
+from tests import test_gpu_adamw as base
+
+pytestmark = pytest.mark.gpu
+
+LR, T, SEED, DECAY = 1e-3, 9, (5 << 32) + 1, [0.01, 0.0, 0.02]
+
+
+class Large(object):
+    """Tensors at addresses off by `shift` elements, with values made on the device."""
+
+    def __init__(self, sizes, bits, gdtype, shift):
+        gen = torch.Generator(device="cuda").manual_seed(bits + shift)
+
+        def put(n, make, dtype=torch.float32):
+            return torch.cat([make(shift), make(n)]).to(dtype)[shift:] if shift else make(n).to(dtype)
+
+        def normal(scale):
+            return lambda n: torch.randn(n, generator=gen, device="cuda") * scale
+
+        def whole(lo, hi):
+            return lambda n: torch.randint(lo, hi, (n,), generator=gen, device="cuda")
+
+        blocks = [(n + 63) // 64 for n in sizes]
+        self.p = [put(n, normal(0.05)) for n in sizes]
+        self.g = [put(n, normal(1e-2), gdtype) for n in sizes]
+        more = {}
+        if bits == 32:
+            self.m = [put(n, normal(3e-3)) for n in sizes]
+            self.v = [put(n, lambda n: normal(1e-2)(n) ** 2) for n in sizes]
+        else:  # any codes that a step can leave
+            self.m = [put(n, lambda n: whole(0, 120)(n) + 128 * whole(0, 2)(n), torch.uint8) for n in sizes]
+            self.v = [put(n, whole(0, 248), torch.uint8) for n in sizes]
+            self.sm = [put(n, whole(110, 125), torch.uint8) for n in blocks]
+            self.sv = [put(n, whole(100, 120), torch.uint8) for n in blocks]
+            more = dict(scale_m=self.sm, scale_v=self.sv)
+        self.opt = AdamW(self.p, self.g, weight_decay=DECAY, state_bits=bits, slot_m=self.m, slot_v=self.v, **more)
+
+
+def places(n):
+    """Starts of runs of 2000 elements: the ends, the middle, and across a chunk's border."""
+    return sorted({0, n // 2 // 64 * 64, 2048 * 64 - 1024, max(0, n - 1000) // 64 * 64} if n > 1 << 18 else {0})
+
+
+@pytest.mark.parametrize("bits,sizes", [(32, [6000001, 1, 3300005]), (8, [12000003, 64, 5100001])])
+@pytest.mark.parametrize("gdtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_steps_past_the_caches_match_the_formula(bits, sizes, gdtype, shift):
+    assert sum(sizes) * (28 if bits == 32 else 16) > 256e6
+    s = Large(sizes, bits, gdtype, shift)
+    before = [[t.clone() for t in x] for x in (s.p, s.g, s.m, s.v)]
+    scales = [[t.clone() for t in x] for x in (s.sm, s.sv)] if bits == 8 else None
+    print("adamw", bits, gdtype, shift, flush=True)
+    s.opt.step(lr=LR, step=T, seed=SEED)
+    torch.cuda.synchronize()
+    f = np.float32
+    for k, n in enumerate(sizes):
+        p, g, m, v = (x[k] for x in before)
+        if bits == 32:
+            g = g.float()
+            assert torch.equal(s.m[k], m * float(f(0.9)) + g * float(f(1 - 0.9)))
+            assert torch.equal(s.v[k], v * float(f(0.999)) + (g * g) * float(f(1 - 0.999)))
+        for at in places(n):
+            part = slice(at, min(n, at + 2000))
+            hp, hg, hm, hv = (t[part].float().cpu().numpy() if t.dtype != torch.uint8 else t[part].cpu().numpy()
+                              for t in (p, g, m, v))
+            if bits == 8:
+                block = slice(at // 64, (part.stop + 63) // 64)
+                hm = base.decode(hm, scales[0][k][block].cpu().numpy(), 16).astype(f)
+                hv = base.decode(hv, scales[1][k][block].cpu().numpy(), 32).astype(f)
+            hm, hv = base.moments(hm, hv, hg)
+            base.check_p(s.p[k][part].cpu().numpy(), hp, hm, hv, LR, DECAY[k], T)
+            if bits == 8:
+                r = base.random_bits(part.stop - at, k, T, SEED, at)
+                done = hm.size // 64 * 64 if part.stop < n else hm.size  # (whole blocks)
+                for codes, scale, x, span, r16 in ((s.m[k], s.sm[k], hm, 16, r & 0xFFFF), (s.v[k], s.sv[k], hv, 32, r >> 16)):
+                    ec, es = base.encode(x, span, (r16 << 4) + 8)
+                    got, whole = codes[part].cpu().numpy(), (done + 63) // 64
+                    assert np.array_equal(scale[block].cpu().numpy()[:whole], es[:whole]), (k, at, span)
+                    same = got == ec
+                    if span == 16:  # (-0 and 0 stand for one value)
+                        same |= (got & 127) + (ec & 127) == 0
+                    assert same[:done].all(), (k, at, span)
