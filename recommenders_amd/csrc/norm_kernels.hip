@@ -218,7 +218,9 @@ __device__ __forceinline__ float exp_of(float u) {
 __device__ __forceinline__ float sigmoid_of(float u) { return __builtin_amdgcn_rcpf(1.f + exp_of(-u)); }
 
 // 1 - 2 / (e^2|u| + 1); below 0.6, where that cancels, u (1 + u^2 P(u^2)) with P interpolated (error 3e-9).  (Here the
-// exponent's rounding needs no correction: it moves the result by less than one unit of the last place.)
+// exponent's rounding needs no correction: it moves the result by less than one unit of the last place.  Slopes over |u| < 6
+// are off by 0.509 x 2^-24 in the mean, 2.26 at most; corrected by 0.502 and 2.21, and 1001 x 4099 fp32 takes 9.7 us
+// instead of 8.7.)
 __device__ __forceinline__ float tanh_of(float u) {
   const float w = u * u;
   float p = fmaf(w, -0.00584964391f, 0.0207513491f);
@@ -230,7 +232,8 @@ __device__ __forceinline__ float tanh_of(float u) {
   return fabsf(u) < 0.6f ? small : large;
 }
 
-// e^u - 1 for u <= 0; above -0.5 u (1 + u Q(u)) with Q interpolated (error 2e-9)
+// e^u - 1 for u <= 0; above -0.5 u (1 + u Q(u)) with Q interpolated (error 2e-9), below without the exponent's correction
+// for tanh's reason (|u| e^u < 0.4: the result moves by half a unit of the last place)
 __device__ __forceinline__ float expm1_of(float u) {
   float q = fmaf(u, 0.00112340425f, 0.00818961363f);
   q = fmaf(u, q, 0.0416300728f);
@@ -242,6 +245,9 @@ __device__ __forceinline__ float expm1_of(float u) {
 // Where a result is stored in 16 bits, and for slopes there, the exponent's own rounding may stay: |u| 2^-24 of the value,
 // 2^-17 at most before the value itself is out of range, a hundredth of the storage's half step and less; a slope is off
 // by less than 2^-24 so (|u| e^-|u| < 0.4).  Half the operations of a sigmoid: 632 x 12980 bf16 11.9 against 14.4 us.
+// Slopes over |u| < 6, off in the mean and at most, in 2^-24: sigmoid 0.228, 1.65 (corrected 0.222, 1.66), tanh 0.516, 2.26
+// (0.502, 2.21), elu 0.046, 0.80 (0.035, 0.80); corrected, 2496 x 16384 bf16 backward takes 55 us instead of 53 with
+// sigmoid, 53.4 and 50.8 with elu, 63 and 53 with tanh, and 409 x 54188 with tanh 50 and 38.5.
 __device__ __forceinline__ float exp_quick(float u) { return __builtin_amdgcn_exp2f(u * 1.44269504f); }
 __device__ __forceinline__ float sigmoid_quick(float u) { return __builtin_amdgcn_rcpf(1.f + exp_quick(-u)); }
 // (up to 0.1 the series, to 2^-23 and 2^-20; from there on 2^-22 of 1 is 2^-18 of the value, a sixtieth of fp16's half
