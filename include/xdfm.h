@@ -788,9 +788,9 @@ int xdfm_bn_bwd_apply(const float* x, const float* y, const float* dy, int64_t B
  *     between consecutive rows, any alignment of the type; what lies between rows is neither read nor
  *     written.  gamma, beta, dgamma, dbeta [cols] and stats are fp32, as is all arithmetic (long sums: wider).
  * Activations and slopes come from the hardware's 2^x and reciprocal.  In units of 2^-24: fp32 results are off by at most
- * 7 of their value (sigmoid, tanh, elu), slopes of every type by 6.6 of 1, and so are the fp32 dgamma and dbeta of one
- * row.  Calls of 16 bits do without the exponent's correction: their results are off, before they are stored, by at most
- * 5 + 1.3 |u| (sigmoid), 50 (tanh) and 24 (elu) of their value (half a step of the type is 2^13 or 2^16).
+ * 7 of their value (sigmoid, tanh, elu), slopes by 6.6 of 1, whatever the type.  Calls of 16 bits do without the
+ * exponent's correction: their results are off, before they are stored, by at most 5 + 1.3 |u| (sigmoid), 50 (tanh) and
+ * 24 (elu) of their value (half a step of the type is 2^13 or 2^16), their slopes within the same 6.6.
  *   stats [2, rows] (NULL ok): mean, then rstd, for the backward pass.
  * A row that holds a NaN or an infinity has no statistics: its y is NaN throughout, under relu too.
  * y may be x (same address and stride); dx may be dy or x.

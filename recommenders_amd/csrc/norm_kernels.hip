@@ -233,7 +233,7 @@ __device__ __forceinline__ float tanh_of(float u) {
 }
 
 // e^u - 1 for u <= 0; above -0.5 u (1 + u Q(u)) with Q interpolated (error 2e-9), below without the exponent's correction
-// for tanh's reason (|u| e^u < 0.4: the result moves by half a unit of the last place)
+// for tanh's reason (|u| e^u < 0.4: the result moves by less than one unit of the last place)
 __device__ __forceinline__ float expm1_of(float u) {
   float q = fmaf(u, 0.00112340425f, 0.00818961363f);
   q = fmaf(u, q, 0.0416300728f);
