@@ -390,8 +390,9 @@ int xdfm_dense_reg_loss(const float* param, int32_t n_seg, const int64_t* seg_of
  * 2^(s - 159) for v: 4 significant bits over 17 binades of m, 33 of v.  Values are rounded up with the
  * probability that the cut-off part is of the last kept bit, out of 16 random bits of (seed, step, tensor's
  * position in the plan, element): to the nearest, a v that moves by a thousandth of itself per step would
- * never move.  A v > 0 never becomes 0.  The step itself uses m and v before they are rounded.  A block with
- * a value that is not finite gets the scale 255 and reads as NaN from then on.
+ * never move.  (A step count read from the device is a float and stays at 2^24: from there on the bits are also those
+ * of the element's gradient and new parameter.)  A v > 0 never becomes 0.  The step itself uses m and v before they are
+ * rounded.  A block with a value that is not finite gets the scale 255 and reads as NaN from then on.
  * ---------------------------------------------------------------------- */
 typedef struct xdfm_adamw_tensor {
   float* param;        /* fp32 [n], device */

@@ -63,12 +63,14 @@ struct Args {
 struct Step {
   float size, inv_root;
   uint32_t t;
+  bool past;  // t is a float that has come to stand still
 };
 
 __device__ __forceinline__ Step step_of(const Args& a) {
-  if (!a.state) return {a.step, a.inv_root, a.t};
+  if (!a.state) return {a.step, a.inv_root, a.t, false};
   const float t = fmaxf(a.state[3], 1.f);  // (a state that was not advanced yet: the first step)
-  return {a.lr / -expm1f(t * a.log_b1), 1.f / sqrtf(-expm1f(t * a.log_b2)), (uint32_t)t};
+  return {a.lr / -expm1f(t * a.log_b1), 1.f / sqrtf(-expm1f(t * a.log_b2)), (uint32_t)t,
+          __builtin_amdgcn_readfirstlane(t >= 0x1p24f) != 0};
 }
 
 // (multiplications and additions are not contracted in this build: m and v are the two products' sum.  Root and
@@ -97,6 +99,10 @@ __device__ __forceinline__ uint32_t random_bits(uint2 k, uint32_t i) {
   a = (a ^ (a >> 15) ^ k.y) * kMul2;
   return a ^ (a >> 16);
 }
+
+// What sets an element's random bits apart from those of other steps once the step count does not: a float stays at 2^24,
+// and with the same bits every step a v that decays by a thousandth of itself would stay where it is (98 of 100 do).
+__device__ __forceinline__ uint32_t salt_of(float p, float g) { return __float_as_uint(p) * kMul1 ^ __float_as_uint(g); }
 
 // largest magnitude of a block (as bits: NaN above infinity above the rest) -> its scale byte
 __device__ __forceinline__ int scale_of(uint32_t top) {
@@ -227,8 +233,9 @@ __device__ __forceinline__ void decode(uint32_t cm, uint32_t cv, int sm, int sv,
 
 // (a whole block's 16 lanes call it; what lies behind a tensor's end is 0 and raises no scale)
 template <bool RANDOM>
-__device__ __forceinline__ void encode(const float (&m)[kEach], const float (&v)[kEach], uint2 key, uint32_t index,
-                                       Four<uint8_t>& cm, Four<uint8_t>& cv, int& sm, int& sv) {
+__device__ __forceinline__ void encode(const float (&m)[kEach], const float (&v)[kEach], uint2 key,
+                                       const uint32_t (&index)[kEach], Four<uint8_t>& cm, Four<uint8_t>& cv, int& sm,
+                                       int& sv) {
   uint32_t am = 0, av = 0;
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
@@ -242,7 +249,7 @@ __device__ __forceinline__ void encode(const float (&m)[kEach], const float (&v)
   for (int j = 0; j < kEach; ++j) {
     uint32_t rm = 1u << 19, rv = 1u << 19;
     if (RANDOM) {
-      const uint32_t r = random_bits(key, index + j);
+      const uint32_t r = random_bits(key, index[j]);
       rm = ((r & 0xFFFFu) << 4) + 8u;
       rv = ((r >> 16) << 4) + 8u;
     }
@@ -310,15 +317,21 @@ __device__ __forceinline__ void step8(const Chunk& c, const Args& a, const Step&
   for (int k = 0; k < N; ++k) {
     const int i = first + k * kThreads * kEach;
     float g[kEach], mj[kEach], vj[kEach];
+    uint32_t index[kEach];
     as_floats(g4[k], g);
     decode(m4[k].w, v4[k].w, sm[k], sv[k], mj, vj);
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       p4[k].w[j] = update(p4[k].w[j], g[j], mj[j], vj[j], a, s, wd);
+      index[j] = (uint32_t)(c.start + i + j);
       if (EDGE && i + j >= c.count) mj[j] = vj[j] = 0.f;  // (a block of NaN is NaN behind the end too)
     }
+    if (s.past) {
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) index[j] ^= salt_of(p4[k].w[j], g[j]);
+    }
     put<EDGE, STREAM>(c.p, i, c.count, p4[k]);
-    encode<true>(mj, vj, key, (uint32_t)(c.start + i), m4[k], v4[k], sm[k], sv[k]);
+    encode<true>(mj, vj, key, index, m4[k], v4[k], sm[k], sv[k]);
     put<EDGE, STREAM>(m, i, c.count, m4[k]);
     put<EDGE, STREAM>(v, i, c.count, v4[k]);
     if ((threadIdx.x & 15) == 0 && (!EDGE || i < c.count)) {
@@ -428,7 +441,7 @@ __global__ __launch_bounds__(kThreads) void adamw_state_write_kernel(const Chunk
     as_floats(get<true, false>(in_v + c.out, i, c.count), v);
     Four<uint8_t> m4, v4;
     int sm, sv;
-    encode<false>(m, v, make_uint2(0, 0), 0, m4, v4, sm, sv);
+    encode<false>(m, v, make_uint2(0, 0), {0u, 0u, 0u, 0u}, m4, v4, sm, sv);
     put<true, false>((uint8_t*)c.m, i, c.count, m4);
     put<true, false>((uint8_t*)c.v, i, c.count, v4);
     if ((threadIdx.x & 15) == 0 && i < c.count) {

@@ -111,7 +111,8 @@ class AdamW(object):
     def step(self, lr, beta1=0.9, beta2=0.999, eps=1e-8, step=None, opt_state=None, seed=0):
         """One step of every tensor on the current stream.  The step count t (from 1) is ``step``, or is read from
         ``opt_state[3]`` on the device (a float tensor kept by ``xdfm_opt_advance``) so that the call can be captured
-        in a HIP graph.  ``seed``: of the rounding of 8-bit states."""
+        in a HIP graph (a float: it stays at 2^24, where t no longer matters to the step; the rounding of 8-bit states
+        goes on by other bits).  ``seed``: of the rounding of 8-bit states."""
         if (step is None) == (opt_state is None):
             raise ValueError("AdamW.step takes either step or opt_state")
         if opt_state is None:

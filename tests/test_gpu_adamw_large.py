@@ -91,3 +91,33 @@ def test_steps_past_the_caches_match_the_formula(bits, sizes, gdtype, shift):
                     if span == 16:  # (-0 and 0 stand for one value)
                         same |= (got & 127) + (ec & 127) == 0
                     assert same[:done].all(), (k, at, span)
+
+
+def test_rounding_goes_on_when_the_devices_step_count_stands_still():
+    """opt_state[3] is a float: 2^24 + 1 is 2^24.  A v of 1 under gradients of some 1e-5 decays by a thousandth a step;
+    rounded by the same bits every step, the 98 of 100 elements that stay once stay for ever.  After 400 steps the mean
+    is 0.999^400 (the gradients add 1e-10).  A step's rounding is off by a code step, a sixteenth under 1, with a
+    probability that the distance 0.001 v gives: a deviation of sqrt(0.001 / 16) at most, of 400 steps 20 times that, of
+    the mean over 4096 elements 64 times less: 0.0025, five of which are allowed."""
+    n = 4096
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    p, g = [torch.randn(n, generator=gen, device="cuda")], [torch.zeros(n, device="cuda")]
+    opt = AdamW(p, g, weight_decay=0.0, state_bits=8)
+    opt.write_state(torch.zeros(n, device="cuda"), torch.ones(n, device="cuda"))
+    state = torch.tensor([0.0, 0.0, 0.0, 2.0 ** 24], device="cuda")
+    for _ in range(400):
+        base._lib.check(base._lib.lib.xdfm_opt_advance(state.data_ptr(), 1e-3, 0.9, 0.999, 1e-8, None,
+                                                       torch.cuda.current_stream().cuda_stream))
+        g[0].copy_(1e-5 * torch.randn(n, generator=gen, device="cuda"))
+        opt.step(lr=1e-3, opt_state=state, seed=7)
+    assert float(state[3]) == 2.0 ** 24
+    v = opt.read_state()[1].double()
+    assert abs(float(v.mean()) - 0.999 ** 400) <= 5 * 0.0025, float(v.mean())
+    # below 2^24 nothing but seed, step, tensor and element counts: another p and g, the same bits
+    a, b = [AdamW([torch.full((n,), 1.0 + k, device="cuda")], [torch.full((n,), 1e-20 * k, device="cuda")],
+                  weight_decay=0.0, state_bits=8) for k in range(2)]
+    below = torch.tensor([0.0, 0.0, 0.0, 2.0 ** 24 - 1], device="cuda")
+    for opt in (a, b):
+        opt.write_state(torch.zeros(n, device="cuda"), torch.linspace(0.5, 1, n, device="cuda"))
+        opt.step(lr=1e-3, opt_state=below, seed=7)
+    assert torch.equal(a.slot_v[0], b.slot_v[0])
