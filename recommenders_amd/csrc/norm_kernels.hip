@@ -10,9 +10,10 @@
 // once and walk the rows, so that gamma, beta and the weights' gradients stay with a thread's columns.
 //   1024 x 65536 fp32 relu, forward     91 us, 5.9 TB/s of 6.2 that a plain streaming addition reaches
 //    512 x 65536 fp32 relu, backward    73 us, 5.5 TB/s, 5 of them in the second launch that joins 256 partial sums
-//   2496 x 16384 bf16, backward         47.5 us, 5.2 TB/s, 5 of them in the second launch
+//   2496 x 16384 bf16, backward         49 us, 5.0 TB/s, 4.7 of them in the second launch
 // Rows that the registers of a block do not hold (16384 elements backward; 18432, of 16 bits 20480, forward) take a slower
-// way (2.2 to 2.9 TB/s).
+// way: 20483 x 533 fp32 29 us forward and 63 backward, 3.0 and 2.1 TB/s; few rows leave CUs idle (400001 x 21 fp32 136 and
+// 215 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -612,7 +613,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void layer_norm_bwd_kernel(
 // 256 registers: they have more bytes under way (80 KB of a CU's reads at 5 pieces) than the sixteen of 8 elements a thread
 // (30 KB), and the sums of a row alone in its wave need no barrier.  What is not needed all the time makes room for that:
 // gamma and beta lie in LDS, xhat is formed again for dx.  us, against the kernel above (beyond 8192 columns: below):
-//   bf16   640 x 16384  16.7, 21.3    2496 x 16384  47.5, 53.5 (with tanh 59, 74)    4346 x 8192  48, 65    8192 x 8192  77, 78
+//   bf16   640 x 16384  16.7, 21.3    2496 x 16384  49, 54 (with tanh 53, 74)    4346 x 8192  48, 65    8192 x 8192  77, 78
 //          12288 x 8192  109, 269     16384 x 64  14.6, 16.7
 //   fp32   640 x 16384  23.2, 25.3    1280 x 4096  15.4, 18.1    1280 x 65536  182, 170    12288 x 8192  212, 460
 constexpr int kRowWaves = 8;
